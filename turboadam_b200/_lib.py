@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libturboadam_b200.so")
 
 TA_OK = 0
 TA_F32, TA_BF16 = 0, 1
+TA_F16 = 2  # the matrix operators only
 TA_M_COSTATE = 1 << 0
 TA_V_ONEQ = 1 << 1
 TA_M_HAS_STATE = 1 << 2
@@ -31,6 +32,11 @@ TA_SHARD_ALIGN_BLOCKS = 4096
 TA_STATUS_NONFINITE_GRAD = 1 << 0
 TA_STATUS_WAIT_TIMEOUT = 1 << 1
 TA_STATUS_BIAS_TABLE_SHORT = 1 << 2
+
+# include/turboadam_b200_matrix.h
+TA_ACT_NONE, TA_ACT_RELU, TA_ACT_GELU, TA_ACT_GELU_TANH, TA_ACT_SILU = range(5)
+TA_ORTHO_UPDATE = 1 << 0
+TA_ORTHO_PAIR = 1 << 1
 
 STATUS_NAMES = {
     1: "TA_ERR_INVALID",
@@ -64,6 +70,15 @@ EXPORTED = (
     "ta_step_prepared",
     "ta_selftest_fast_math",
     "ta_selftest_wait_timeout",
+)
+# Every symbol declared in include/turboadam_b200_matrix.h.
+MATRIX_EXPORTED = (
+    "ta_ortho_workspace_size",
+    "ta_orthogonalize",
+    "ta_linear_workspace_size",
+    "ta_linear_forward",
+    "ta_linear_backward_workspace_size",
+    "ta_linear_backward",
 )
 
 
@@ -127,6 +142,76 @@ class TaDynamic(ctypes.Structure):
         ("lr_dev", ctypes.c_void_p),
         ("grad_scale_dev", ctypes.c_void_p),
         ("found_inf_dev", ctypes.c_void_p),
+    ]
+
+
+class TaOrthoTensor(ctypes.Structure):
+    _fields_ = [
+        ("in_dev", ctypes.c_void_p),
+        ("momentum_dev", ctypes.c_void_p),
+        ("out_dev", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("in_dtype", ctypes.c_int32),
+        ("momentum_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+        ("keep", ctypes.c_double),
+        ("gain", ctypes.c_double),
+    ]
+
+
+class TaOrthoOptions(ctypes.Structure):
+    _fields_ = [
+        ("coefficients", ctypes.c_void_p),
+        ("steps", ctypes.c_int32),
+        ("nesterov", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+        ("momentum", ctypes.c_double),
+    ]
+
+
+class TaLinear(ctypes.Structure):
+    _fields_ = [
+        ("x_dev", ctypes.c_void_p),
+        ("w_dev", ctypes.c_void_p),
+        ("bias_dev", ctypes.c_void_p),
+        ("residual_dev", ctypes.c_void_p),
+        ("y_dev", ctypes.c_void_p),
+        ("deriv_dev", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("fan_in", ctypes.c_int64),
+        ("fan_out", ctypes.c_int64),
+        ("x_strides", ctypes.c_int64 * 2),
+        ("w_strides", ctypes.c_int64 * 2),
+        ("residual_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class TaLinearGrad(ctypes.Structure):
+    _fields_ = [
+        ("dy_dev", ctypes.c_void_p),
+        ("deriv_dev", ctypes.c_void_p),
+        ("x_dev", ctypes.c_void_p),
+        ("w_dev", ctypes.c_void_p),
+        ("dx_dev", ctypes.c_void_p),
+        ("dw_dev", ctypes.c_void_p),
+        ("db_dev", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("fan_in", ctypes.c_int64),
+        ("fan_out", ctypes.c_int64),
+        ("dy_stride", ctypes.c_int64),
+        ("x_strides", ctypes.c_int64 * 2),
+        ("w_strides", ctypes.c_int64 * 2),
+        ("dw_strides", ctypes.c_int64 * 2),
+        ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
     ]
 
 
@@ -197,6 +282,12 @@ _SIG = {
                                         _P, ctypes.c_size_t, ctypes.POINTER(TaDynamic), _P]),
     "ta_selftest_fast_math": (ctypes.c_int, [_P, _P]),
     "ta_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_uint64, _P, _P, _P]),
+    "ta_ortho_workspace_size": (ctypes.c_size_t, [_P, ctypes.c_int32, _P]),
+    "ta_orthogonalize": (ctypes.c_int, [_P, ctypes.c_int32, _P, _P, ctypes.c_size_t, _P, _P]),
+    "ta_linear_workspace_size": (ctypes.c_size_t, [_P]),
+    "ta_linear_forward": (ctypes.c_int, [_P, _P, ctypes.c_size_t, _P, _P]),
+    "ta_linear_backward_workspace_size": (ctypes.c_size_t, [_P]),
+    "ta_linear_backward": (ctypes.c_int, [_P, _P, ctypes.c_size_t, _P, _P]),
 }
 
 _lib = None

@@ -2,9 +2,12 @@
 
     python -m turboadam_b200.csrc.build [--verbose-ptxas]
 
-Flags that make the device arithmetic bit-identical to the host checker:
---fmad=false (no a*b+c contraction; the sources call __fmaf_rn explicitly
-where torch fuses), IEEE division and square root, no flush-to-zero.
+Each source is compiled to an object of its own (csrc/_build/, rebuilt when
+the source or a header it includes is newer) and the objects are linked.
+
+Flags that make the packed step's device arithmetic bit-identical to the host
+checker: --fmad=false (no a*b+c contraction; the sources call __fmaf_rn
+explicitly where torch fuses), IEEE division and square root, no flush-to-zero.
 """
 from __future__ import annotations
 
@@ -17,10 +20,26 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 OUT = os.path.join(PKG, "libturboadam_b200.so")
-SOURCES = [os.path.join(HERE, "ta_api.cu")]
-DEPS = SOURCES + [os.path.join(HERE, f) for f in
-                  ("ta_kernels.cuh", "ta_codec.cuh", "ta_device.cuh", "ta_math.h")] + [
-    os.path.join(os.path.dirname(PKG), "include", "turboadam_b200.h")]
+OBJ_DIR = os.path.join(HERE, "_build")
+INCLUDE = os.path.join(os.path.dirname(PKG), "include")
+
+
+def _paths(*names):
+    return [os.path.join(HERE, f) for f in names]
+
+
+# source -> the headers it includes
+UNITS = {
+    os.path.join(HERE, "ta_api.cu"):
+        _paths("ta_kernels.cuh", "ta_codec.cuh", "ta_device.cuh", "ta_math.h", "ta_host.h")
+        + [os.path.join(INCLUDE, "turboadam_b200.h")],
+    os.path.join(HERE, "ta_mx_api.cu"):
+        _paths("ta_mx_device.cuh", "ta_mx_product.cuh", "ta_mx_elementwise.cuh", "ta_host.h")
+        + [os.path.join(INCLUDE, "turboadam_b200.h"),
+           os.path.join(INCLUDE, "turboadam_b200_matrix.h")],
+}
+SOURCES = list(UNITS)
+DEPS = sorted({f for src, heads in UNITS.items() for f in [src, *heads]})
 
 
 def nvcc() -> str:
@@ -50,11 +69,37 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(d) <= t for d in DEPS)
 
 
+def _object(src: str) -> str:
+    return os.path.join(OBJ_DIR, os.path.splitext(os.path.basename(src))[0] + ".o")
+
+
+def _stale(src: str) -> bool:
+    obj = _object(src)
+    if not os.path.exists(obj):
+        return True
+    t = os.path.getmtime(obj)
+    return any(os.path.getmtime(d) > t for d in [src, *UNITS[src]])
+
+
 def build(force: bool = False, ptxas_verbose: bool = False, quiet: bool = False) -> str:
     if not force and up_to_date():
         return OUT
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    base = [f for f in flags(ptxas_verbose) if f != "-shared"]
+    jobs = []
+    for src in SOURCES:
+        if force or _stale(src):
+            tmp = _object(src) + ".tmp.o"
+            cmd = [nvcc()] + base + ["-c", "-o", tmp, src]
+            if not quiet:
+                print(" ".join(cmd), flush=True)
+            jobs.append((src, tmp, cmd, subprocess.Popen(cmd)))
+    for src, tmp, cmd, job in jobs:
+        if job.wait() != 0:
+            raise subprocess.CalledProcessError(job.returncode, cmd)
+        os.replace(tmp, _object(src))
     tmp = OUT + ".tmp"
-    cmd = [nvcc()] + flags(ptxas_verbose) + ["-o", tmp] + SOURCES
+    cmd = [nvcc()] + flags() + ["-o", tmp] + [_object(src) for src in SOURCES]
     if not quiet:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)

@@ -14,6 +14,7 @@
 
 #include "../../include/turboadam_b200.h"
 #include "ta_codec.cuh"
+#include "ta_host.h"
 #include "ta_kernels.cuh"
 
 using namespace ta;
@@ -22,10 +23,7 @@ namespace {
 
 thread_local std::string g_err;
 
-ta_status fail(ta_status s, const std::string& m) {
-  g_err = m;
-  return s;
-}
+ta_status fail(ta_status s, const std::string& m) { return ta_fail(s, m); }
 
 #define TA_CU(x)                                                                  \
   do {                                                                            \
@@ -659,6 +657,11 @@ ta_status run_step(const ta_tensor* ts, int nT, const ta_group* groups, uint64_t
 }
 
 }  // namespace
+
+ta_status ta_fail(ta_status s, const std::string& message) {
+  g_err = message;
+  return s;
+}
 
 extern "C" {
 

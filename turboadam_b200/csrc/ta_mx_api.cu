@@ -1,0 +1,991 @@
+// ta_mx_api.cu -- host side of the matrix operators (include/turboadam_b200_matrix.h):
+// argument validation, operand tensor maps, the choice of tile and split, workspace
+// layout and the launch sequences.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <string>
+#include <utility>
+#include <vector>
+
+#include "../../include/turboadam_b200_matrix.h"
+#include "ta_host.h"
+#include "ta_mx_elementwise.cuh"
+#include "ta_mx_product.cuh"
+
+using namespace ta::mx;
+
+namespace {
+
+#define MX_CU(x)                                                                        \
+  do {                                                                                  \
+    cudaError_t e_ = (x);                                                               \
+    if (e_ != cudaSuccess)                                                              \
+      return ta_fail(TA_ERR_CUDA, std::string(#x) + ": " + cudaGetErrorString(e_));     \
+  } while (0)
+#define MX_OK(x)                  \
+  do {                            \
+    ta_status s_ = (x);           \
+    if (s_ != TA_OK) return s_;   \
+  } while (0)
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t up8(int64_t x) { return (x + 7) & ~(int64_t)7; }
+inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+inline int64_t dt_bytes(int dt) { return dt == TA_F32 ? 4 : 2; }
+
+constexpr int64_t kMaxDim = 0x7fffff00;  // every dimension (rows, columns) is held in 32 bits
+
+int sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
+// ---- workspace -------------------------------------------------------------
+// Hands out 256-byte aligned pieces; with a null base it only measures.
+struct Arena {
+  uint8_t* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t count) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += al256(count * sizeof(T));
+    return p;
+  }
+};
+
+// ---- tensor maps -------------------------------------------------------------
+using EncodeFn = decltype(&cuTensorMapEncodeTiled);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// The tensor-map encoder is a driver call: it needs the device's context to be current on the
+// calling thread, which on a fresh thread (autograd's, say) only a runtime call makes it.
+ta_status bind_device() {
+  int dev = 0;
+  MX_CU(cudaGetDevice(&dev));
+  MX_CU(cudaSetDevice(dev));
+  return TA_OK;
+}
+
+// An operand of a product: `mn` output rows (or columns) by `k`, 16-bit elements, one of the two
+// contiguous; lines of the other are ld elements apart, matrices zs elements apart.
+struct Operand {
+  const void* p = nullptr;
+  int64_t mn = 0, k = 0, ld = 0, zs = 0, z = 1;
+  bool mn_major = false;
+};
+
+ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return ta_fail(TA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const int64_t inner = o.mn_major ? o.mn : o.k, lines = o.mn_major ? o.k : o.mn;
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)lines, (cuuint64_t)o.z};
+  cuuint64_t strides[2] = {(cuuint64_t)(o.ld * 2),
+                           (cuuint64_t)(std::max<int64_t>(o.zs, o.ld) * 2)};
+  cuuint32_t box[3] = {64, (cuuint32_t)(o.mn_major ? kDepth : kRows), 1};
+  cuuint32_t step[3] = {1, 1, 1};
+  CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(o.p), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return ta_fail(TA_ERR_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string((int)r));
+  return TA_OK;
+}
+
+// ---- one launch of the tile engine -----------------------------------------------
+struct Product {
+  Operand a, b;
+  int64_t M = 0, N = 0;
+  int parts = 1;
+  bool sym = false;
+  int64_t batch = 1;
+  Problem ep;  // the epilogue's fields
+  Product() { memset(&ep, 0, sizeof(ep)); }
+};
+
+int64_t tiles_of(const Product& p, int cg, int* tm = nullptr, int* tn = nullptr) {
+  const int64_t side = 128 * cg, m = cdiv(p.M, side), n = cdiv(p.N, side);
+  if (tm) *tm = (int)m;
+  if (tn) *tn = (int)n;
+  return p.sym ? m * (m + 1) / 2 : m * n;
+}
+int64_t blocks_of(const Product& p) { return cdiv(p.a.k, kDepth) * p.parts; }
+
+struct Shape {
+  int cg = 1;
+  std::vector<int> splits;
+};
+
+constexpr int64_t kSplitUnits = 296;  // room for the split tiles of one launch
+constexpr size_t kSplitTileBytes = (size_t)kRows * 128 * 4;
+
+// Tile and splits of a launch. The large tile runs at the tensor pipe's rate and the small one
+// at about 0.85 of it (shared-memory bandwidth), so the small one is for lists whose large tiles
+// would leave pairs of SMs idle: the lower estimate of (rounds of tiles) x (time of a tile) wins.
+// Where even the small tiles do not fill the SMs, sums of 8 or more k blocks are split until
+// they do.
+Shape choose(const std::vector<Product>& ps) {
+  const int sms = sm_count();
+  int64_t u1 = 0, u2 = 0, w1 = 0, w2 = 0, longest = 0;
+  for (const Product& p : ps) {
+    const int64_t kb = std::max<int64_t>(1, blocks_of(p));
+    const int64_t t1 = tiles_of(p, 1) * p.batch, t2 = tiles_of(p, 2) * p.batch;
+    u1 += t1;
+    u2 += t2;
+    w1 += t1 * kb;
+    w2 += t2 * kb;
+    longest = std::max(longest, kb);
+  }
+  Shape s;
+  s.splits.assign(ps.size(), 1);
+  if (u1 == 0) return s;
+  const double rounds1 = (double)cdiv(u1, sms), rounds2 = (double)cdiv(u2, sms / 2);
+  const double time2 = std::max(rounds2 * (double)w2 / (double)u2, (double)longest) * 2.0;
+  const bool split = u1 * 2 <= sms && longest >= 16;
+  const double time1 =
+      (split ? (double)w1 / sms + 8 : std::max(rounds1 * (double)w1 / (double)u1, (double)longest)) *
+      1.18;
+  if (time2 <= time1) {
+    s.cg = 2;
+    return s;
+  }
+  if (split) {
+    const double ideal = std::max(8.0, (double)w1 / sms);
+    int64_t units = 0;
+    for (size_t i = 0; i < ps.size(); ++i) {
+      const int64_t kb = blocks_of(ps[i]);
+      s.splits[i] = (int)std::max<int64_t>(1, std::min<int64_t>(32, (int64_t)(kb / ideal)));
+      if (s.splits[i] > 1) units += tiles_of(ps[i], 1) * ps[i].batch * s.splits[i];
+    }
+    if (units > kSplitUnits) s.splits.assign(ps.size(), 1);
+  }
+  return s;
+}
+
+// Shared-memory limit and resident CTAs (or CTA pairs) of an instance, found once per device. A
+// die's SM count need not divide into pairs, so the pairs that fit are asked for: a pair that had
+// to wait for another to finish would double the time of a persistent launch.
+template <int CG, int EPI>
+ta_status workers_of(int* workers) {
+  constexpr int kMaxDevices = 64;
+  static std::mutex m;
+  static int found[kMaxDevices] = {};
+  int dev = 0;
+  MX_CU(cudaGetDevice(&dev));
+  if (dev >= kMaxDevices) return ta_fail(TA_ERR_UNSUPPORTED, "device index over 63");
+  std::lock_guard<std::mutex> lock(m);
+  if (!found[dev]) {
+    MX_CU(cudaFuncSetAttribute(k_product<CG, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)kProductSmem));
+    int n = sm_count();
+    if (CG == 2) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 2;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.gridDim = dim3((unsigned)(n / 2 * 2));
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = kProductSmem;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      MX_CU(cudaOccupancyMaxActiveClusters(&n, k_product<CG, EPI>, &cfg));
+    }
+    if (n < 1) return ta_fail(TA_ERR_CUDA, "the product kernel does not fit this device");
+    found[dev] = n;
+  }
+  *workers = found[dev];
+  return TA_OK;
+}
+
+template <int CG, int EPI>
+ta_status launch_product(const ProductArgs& g, cudaStream_t stream) {
+  int workers = 0;
+  MX_OK((workers_of<CG, EPI>(&workers)));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(g.units, workers)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kProductSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;
+  if (CG == 2) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  MX_CU(cudaLaunchKernelEx(&cfg, k_product<CG, EPI>, g));
+  return TA_OK;
+}
+
+struct Scalars {
+  float alpha = 1.f, c0 = 0.f, c1 = 0.f, c2 = 0.f;
+  int unit_pow = 0;
+};
+
+// split_ws / split_count: room for kSplitUnits tiles and counters (zero).
+template <int EPI>
+ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars& sc,
+                       float* split_ws, uint32_t* split_count, uint32_t* status,
+                       cudaStream_t stream) {
+  for (size_t lo = 0; lo < all.size(); lo += kMaxProblems) {
+    const std::vector<Product> ps(all.begin() + lo,
+                                  all.begin() + std::min(all.size(), lo + kMaxProblems));
+    MX_OK(bind_device());
+    Shape shape = choose(ps);
+    ProductArgs g;
+    memset(&g, 0, sizeof(g));
+    g.count = (int)ps.size();
+    g.bf16 = bf16;
+    g.alpha = sc.alpha;
+    g.c0 = sc.c0;
+    g.c1 = sc.c1;
+    g.c2 = sc.c2;
+    g.unit_pow = sc.unit_pow;
+    g.status = status;
+    int64_t units = 0, split_units = 0, split_tiles = 0;
+    for (size_t i = 0; i < ps.size(); ++i) {
+      const Product& p = ps[i];
+      Problem& P = g.p[i];
+      P = p.ep;
+      if (p.a.k > 0) {
+        MX_OK(make_map(&P.ta, p.a, bf16));
+        MX_OK(make_map(&P.tb, p.b, bf16));
+      }
+      P.M = (int32_t)p.M;
+      P.N = (int32_t)p.N;
+      P.kblocks = (int32_t)cdiv(p.a.k, kDepth);
+      P.parts = p.parts;
+      P.tiles = (int32_t)tiles_of(p, shape.cg, &P.tiles_m, &P.tiles_n);
+      P.first = (int32_t)units;
+      P.batch = (int32_t)p.batch;
+      P.splits = shape.splits[i];
+      P.a_mn = p.a.mn_major;
+      P.b_mn = p.b.mn_major;
+      P.sym = p.sym;
+      const int64_t tiles = (int64_t)P.tiles * p.batch;
+      if (P.splits > 1) {
+        P.split_ws = split_ws + split_units * (kSplitTileBytes / 4);
+        P.split_count = split_count + split_tiles;
+        split_units += tiles * P.splits;
+        split_tiles += tiles;
+      }
+      units += tiles * P.splits;
+    }
+    if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
+    if (units == 0) continue;
+    g.units = (int32_t)units;
+    if (shape.cg == 2) MX_OK((launch_product<2, EPI>(g, stream)));
+    else MX_OK((launch_product<1, EPI>(g, stream)));
+  }
+  return TA_OK;
+}
+
+// ---- orthogonalisation -----------------------------------------------------------
+// Scales of the fp16 matrices: X, the Gram matrix and the polynomial are at most a few units in
+// norm (the quintic keeps singular values below 1.3), so 2^10 and 2^8 leave 2^6 to 2^8 of head
+// room under fp16's largest number and put elements of 2^-24 and 2^-22 on its smallest normal.
+constexpr float kScaleX = 1024.f, kScaleA = 1024.f, kScaleP = 256.f;
+
+struct Class {  // matrices of one shape
+  int64_t rows = 0, cols = 0, ld = 0, side = 0, lds = 0, count = 0;
+  int first = 0;  // first table slot
+  bool pair = false, tall = false;
+  __half *x0 = nullptr, *x1 = nullptr, *gram = nullptr, *poly = nullptr, *prod = nullptr;
+  int64_t xs() const { return rows * ld; }
+  int64_t ss() const { return side * lds; }
+};
+
+struct OrthoPlan {
+  std::vector<Class> classes;
+  std::vector<std::vector<int>> members;  // tensors of each class
+  int64_t items = 0;
+  int64_t chunks = 0;
+};
+
+int64_t chunk_elems(int64_t n) {
+  return std::max<int64_t>(8192, cdiv(cdiv(n, kMaxChunks), 2048) * 2048);
+}
+
+ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_options* o,
+                     OrthoPlan* plan) {
+  if (n < 0 || (n > 0 && !ts)) return ta_fail(TA_ERR_INVALID, "null tensor list");
+  if (!o || !o->coefficients) return ta_fail(TA_ERR_INVALID, "null options or coefficients");
+  if (o->steps < 1 || o->steps > 32) return ta_fail(TA_ERR_INVALID, "steps must be 1 to 32");
+  if (!(o->eps >= 0)) return ta_fail(TA_ERR_INVALID, "eps must not be negative");
+  std::map<std::pair<std::pair<int64_t, int64_t>, bool>, int> index;
+  for (int i = 0; i < n; ++i) {
+    const ta_ortho_tensor& t = ts[i];
+    auto bad = [&](const char* what) {
+      return ta_fail(TA_ERR_INVALID, "matrix " + std::to_string(i) + ": " + what);
+    };
+    if (t.batch < 0 || t.rows < 0 || t.cols < 0) return bad("negative size");
+    if (t.batch == 0 || t.rows == 0 || t.cols == 0) continue;
+    if (t.rows > kMaxDim || t.cols > kMaxDim || t.batch > kMaxDim)
+      return ta_fail(TA_ERR_UNSUPPORTED,
+                     "matrix " + std::to_string(i) + ": a size is over 2^31 - 256");
+    if (!t.in_dev || !t.out_dev) return bad("null pointer");
+    for (int dt : {t.in_dtype, t.out_dtype, t.momentum_dev ? t.momentum_dtype : (int)TA_F32})
+      if (dt != TA_F32 && dt != TA_BF16 && dt != TA_F16)
+        return bad("dtypes must be TA_F32, TA_BF16 or TA_F16");
+    if ((uintptr_t)t.in_dev % dt_bytes(t.in_dtype) || (uintptr_t)t.out_dev % dt_bytes(t.out_dtype) ||
+        (t.momentum_dev && (uintptr_t)t.momentum_dev % dt_bytes(t.momentum_dtype)))
+      return ta_fail(TA_ERR_ALIGN,
+                     "matrix " + std::to_string(i) + ": pointer not aligned to its type");
+    const bool pair = (t.flags & TA_ORTHO_PAIR) && t.in_dtype == TA_F32;
+    auto key = std::make_pair(std::make_pair(t.rows, t.cols), pair);
+    auto it = index.find(key);
+    if (it == index.end()) {
+      it = index.emplace(key, (int)plan->classes.size()).first;
+      Class c;
+      c.rows = t.rows;
+      c.cols = t.cols;
+      c.ld = up8(t.cols);
+      c.tall = t.rows > t.cols;
+      c.side = std::min(t.rows, t.cols);
+      c.lds = up8(c.side);
+      c.pair = pair;
+      plan->classes.push_back(c);
+      plan->members.emplace_back();
+    }
+    plan->classes[it->second].count += t.batch;
+    plan->members[it->second].push_back(i);
+  }
+  for (Class& c : plan->classes) {
+    c.first = (int)plan->items;
+    plan->items += c.count;
+    plan->chunks += c.count * cdiv(c.rows * c.cols, chunk_elems(c.rows * c.cols));
+    if (plan->items > 0x7fffffff || plan->chunks > 0x7fffffff)
+      return ta_fail(TA_ERR_UNSUPPORTED, "too many matrices in one call");
+  }
+  return TA_OK;
+}
+
+struct OrthoSpace {
+  Item* table;
+  Scale* scale;
+  double* partial;
+  uint32_t* split_count;
+  float* split_ws;
+};
+
+OrthoSpace carve_ortho(OrthoPlan* plan, Arena* a) {
+  OrthoSpace s;
+  s.table = a->take<Item>(plan->items);
+  s.scale = a->take<Scale>(plan->items);
+  s.partial = a->take<double>(plan->chunks);
+  s.split_count = a->take<uint32_t>(kSplitUnits);
+  s.split_ws = a->take<float>(kSplitUnits * kSplitTileBytes / 4);
+  for (Class& c : plan->classes) {
+    c.x0 = a->take<__half>(c.xs() * c.count * (c.pair ? 2 : 1));
+    c.x1 = a->take<__half>(c.xs() * c.count);
+    c.gram = a->take<__half>(c.ss() * c.count);
+    c.poly = a->take<__half>(c.ss() * c.count);
+    c.prod = a->take<__half>(c.ss() * c.count);
+  }
+  return s;
+}
+
+ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoPlan& plan,
+                    const OrthoSpace& sp, uint32_t* status, cudaStream_t stream) {
+  // the table
+  std::vector<ItemSeed> seeds;
+  int64_t chunk = 0;
+  for (size_t k = 0; k < plan.classes.size(); ++k) {
+    const Class& c = plan.classes[k];
+    const int64_t n = c.rows * c.cols, ce = chunk_elems(n), stored = c.xs() * (c.pair ? 2 : 1);
+    int64_t slot = c.first;
+    for (int i : plan.members[k]) {
+      const ta_ortho_tensor& t = ts[i];
+      ItemSeed s;
+      memset(&s, 0, sizeof(s));
+      s.it.g = t.in_dev;
+      s.it.mom = t.momentum_dev;
+      s.it.out = t.out_dev;
+      s.it.x0 = c.x0 + (slot - c.first) * stored;
+      s.it.x0_lo = c.pair ? s.it.x0 + c.xs() : nullptr;
+      s.it.n = n;
+      s.it.cols = (int32_t)c.cols;
+      s.it.ld = (int32_t)c.ld;
+      s.it.chunk0 = (int32_t)chunk;
+      s.it.chunks = (int32_t)cdiv(n, ce);
+      s.it.chunk_elems = ce;
+      s.it.keep = (float)t.keep;
+      s.it.gain = (float)t.gain;
+      s.it.g_dt = (int16_t)t.in_dtype;
+      s.it.mom_dt = (int16_t)t.momentum_dtype;
+      s.it.out_dt = (int16_t)t.out_dtype;
+      s.it.update = (t.flags & TA_ORTHO_UPDATE) != 0;
+      s.first = (int32_t)slot;
+      s.batch = (int32_t)t.batch;
+      s.elem_zs = n;
+      s.x0_zs = stored;
+      seeds.push_back(s);
+      slot += t.batch;
+      chunk += t.batch * s.it.chunks;
+    }
+  }
+  for (size_t lo = 0; lo < seeds.size(); lo += kSeeds) {
+    TableArgs ta;
+    memset(&ta, 0, sizeof(ta));
+    ta.count = (int32_t)std::min<size_t>(kSeeds, seeds.size() - lo);
+    std::copy(seeds.begin() + lo, seeds.begin() + lo + ta.count, ta.s);
+    ta.table = sp.table;
+    ta.scale = sp.scale;
+    ta.partial = sp.partial;
+    ta.zero = sp.split_count;
+    ta.zero_words = lo == 0 ? (int32_t)kSplitUnits : 0;
+    int64_t most = 1;
+    for (int i = 0; i < ta.count; ++i) most = std::max<int64_t>(most, ta.s[i].batch);
+    k_table<<<(unsigned)std::min<int64_t>(cdiv(most, kEltThreads), 64), kEltThreads, 0, stream>>>(ta);
+    MX_CU(cudaGetLastError());
+  }
+  const float mu = (float)o->momentum;
+  k_norm<<<(unsigned)chunk, kEltThreads, 0, stream>>>(sp.table, (int)plan.items, mu, o->nesterov);
+  MX_CU(cudaGetLastError());
+  k_scale<<<(unsigned)chunk, kEltThreads, 0, stream>>>(sp.table, (int)plan.items, mu, o->nesterov,
+                                                      o->eps);
+  MX_CU(cudaGetLastError());
+
+  const size_t nc = plan.classes.size();
+  auto square = [](const Class& c, const __half* p) {
+    Operand q;
+    q.p = p;
+    q.mn = q.k = c.side;
+    q.ld = c.lds;
+    q.zs = c.ss();
+    q.z = c.count;
+    return q;
+  };
+  // the iterate as an operand: rows x cols, row-major, so its columns are contiguous
+  auto iterate = [](const Class& c, const __half* p, bool sum_over_rows, int64_t z) {
+    Operand q;
+    q.p = p;
+    q.mn = sum_over_rows ? c.cols : c.rows;
+    q.k = sum_over_rows ? c.rows : c.cols;
+    q.ld = c.ld;
+    q.zs = c.xs();
+    q.z = z;
+    q.mn_major = sum_over_rows;
+    return q;
+  };
+  // out = left * right of side x side matrices (or the Gram matrix of the iterate), symmetric
+  auto gram = [&](bool first) {  // A from X; the first iterate is x0 (its upper half, if a pair)
+    std::vector<Product> ps;
+    for (const Class& c : plan.classes) {
+      Product p;
+      const bool pair = c.pair && first;
+      p.a = iterate(c, first ? c.x0 : c.x1, c.tall, c.count * (pair ? 2 : 1));
+      p.b = p.a;
+      p.M = p.N = c.side;
+      p.sym = true;
+      p.batch = c.count;
+      p.ep.za = p.ep.zb = pair ? 2 : 1;
+      p.ep.out = c.gram;
+      p.ep.out_zs = c.ss();
+      p.ep.ldo = (int32_t)c.lds;
+      p.ep.scale = sp.scale + c.first;
+      ps.push_back(p);
+    }
+    return ps;
+  };
+  auto squares = [&](int which) {  // 0: the polynomial from A; 1: its product with the last one
+    std::vector<Product> ps;
+    for (const Class& c : plan.classes) {
+      Product p;
+      p.a = square(c, which == 0 ? c.gram : c.poly);
+      p.b = square(c, which == 0 ? c.gram : c.prod);
+      p.M = p.N = c.side;
+      p.sym = true;
+      p.batch = c.count;
+      p.ep.za = p.ep.zb = 1;
+      p.ep.out = which == 0 ? c.poly : c.gram;
+      p.ep.out_zs = c.ss();
+      p.ep.ldo = (int32_t)c.lds;
+      p.ep.aux = c.gram;
+      p.ep.aux_zs = c.ss();
+      p.ep.ld_aux = (int32_t)c.lds;
+      p.ep.scale = sp.scale + c.first;
+      ps.push_back(p);
+    }
+    return ps;
+  };
+  // X <- poly * x (x * poly, if tall); from_x0: x is the scaled input, with both parts of a pair
+  // if `whole`
+  auto apply = [&](const std::vector<__half*>& poly, const std::vector<__half*>& x, bool from_x0,
+                   bool whole, const std::vector<__half*>& out) {
+    std::vector<Product> ps;
+    for (size_t i = 0; i < nc; ++i) {
+      const Class& c = plan.classes[i];
+      Product p;
+      const bool pair = c.pair && from_x0;
+      const Operand q = square(c, poly[i]);
+      const Operand v = iterate(c, x[i], !c.tall, c.count * (pair ? 2 : 1));
+      p.a = c.tall ? v : q;
+      p.b = c.tall ? q : v;
+      p.parts = pair && whole ? 2 : 1;
+      p.M = c.rows;
+      p.N = c.cols;
+      p.batch = c.count;
+      p.ep.za = c.tall && pair ? 2 : 1;
+      p.ep.zb = !c.tall && pair ? 2 : 1;
+      p.ep.out = out[i];
+      p.ep.out_zs = c.xs();
+      p.ep.ldo = (int32_t)c.ld;
+      p.ep.scale = sp.scale + c.first;
+      p.ep.items = sp.table + c.first;
+      ps.push_back(p);
+    }
+    return ps;
+  };
+
+  std::vector<__half*> x0(nc), x1(nc), polys(nc), prods(nc), grams(nc);
+  auto refresh = [&] {
+    for (size_t i = 0; i < nc; ++i) {
+      x0[i] = plan.classes[i].x0;
+      x1[i] = plan.classes[i].x1;
+      polys[i] = plan.classes[i].poly;
+      prods[i] = plan.classes[i].prod;
+      grams[i] = plan.classes[i].gram;
+    }
+  };
+  for (int step = 0; step < o->steps; ++step) {
+    const double* abc = o->coefficients + 3 * step;
+    const bool last = step == o->steps - 1;
+    Scalars sc;
+    // A
+    if (step == 0) {
+      sc.alpha = kScaleA;
+      sc.unit_pow = 2;
+    } else {
+      sc.alpha = kScaleA / (kScaleX * kScaleX);
+    }
+    MX_OK(run_products<EPI_GRAM>(gram(step == 0), false, sc, sp.split_ws, sp.split_count, status,
+                                 stream));
+    // a I + b A + c A^2
+    sc = Scalars();
+    sc.c0 = (float)(kScaleP * abc[0]);
+    sc.c1 = (float)(kScaleP * abc[1] / kScaleA);
+    sc.c2 = (float)(kScaleP * abc[2] / ((double)kScaleA * kScaleA));
+    MX_OK(run_products<EPI_POLY>(squares(0), false, sc, sp.split_ws, sp.split_count, status,
+                                 stream));
+    refresh();
+    // The first two polynomials act on the unrounded input together: the first iterate, rounded,
+    // only serves the second Gram matrix, whose rounding the result hardly feels.
+    std::vector<__half*> poly = polys, x = x1;
+    const bool from_x0 = step <= 1;
+    if (step == 1) {
+      sc = Scalars();
+      sc.alpha = 1.f / kScaleP;
+      MX_OK(run_products<EPI_GRAM>(squares(1), false, sc, sp.split_ws, sp.split_count, status,
+                                   stream));
+      poly = grams;
+    }
+    if (from_x0) x = x0;
+    sc = Scalars();
+    sc.unit_pow = from_x0 ? 1 : 0;
+    if (last) {
+      sc.alpha = from_x0 ? 1.f / kScaleP : 1.f / (kScaleP * kScaleX);
+      MX_OK(run_products<EPI_FINAL>(apply(poly, x, from_x0, true, x1), false, sc, sp.split_ws,
+                                    sp.split_count, status, stream));
+    } else {
+      sc.alpha = from_x0 ? kScaleX / kScaleP : 1.f / kScaleP;
+      // the iterate moves to x1; from the third step on its old storage takes the next one
+      if (step >= 2)
+        for (Class& c : plan.classes) std::swap(c.x0, c.x1);
+      refresh();
+      MX_OK(run_products<EPI_APPLY>(apply(poly, x, from_x0, step == 1, x1), false, sc,
+                                    sp.split_ws, sp.split_count, status, stream));
+      if (step == 0)
+        for (Class& c : plan.classes) std::swap(c.poly, c.prod);
+    }
+  }
+  return TA_OK;
+}
+
+// ---- linear layer ----------------------------------------------------------------
+// A 16-bit matrix given by its two strides, as an operand: TMA reads it where it lies if the
+// lines start on 16 bytes, else it is copied into aligned lines.
+struct Lines {
+  bool mn_major = false;  // the mn dimension is contiguous
+  int64_t lines = 0, len = 0, stride = 0;
+  bool direct = false;
+};
+
+bool lines_of(const void* p, int64_t mn, int64_t k, int64_t s_mn, int64_t s_k, Lines* l) {
+  if (s_k == 1 || k <= 1) {
+    l->mn_major = false;
+    l->lines = mn;
+    l->len = k;
+    l->stride = s_mn;
+  } else if (s_mn == 1 || mn <= 1) {
+    l->mn_major = true;
+    l->lines = k;
+    l->len = mn;
+    l->stride = s_k;
+  } else {
+    return false;
+  }
+  if (l->lines <= 1) l->stride = up8(l->len);
+  l->direct = aligned16(p) && l->stride % 8 == 0 && l->stride >= l->len;
+  return l->lines <= 1 || l->stride >= l->len;
+}
+
+ta_status operand_of(const void* p, int64_t mn, int64_t k, const Lines& l, uint16_t* copy,
+                     Operand* o, cudaStream_t stream) {
+  o->mn = mn;
+  o->k = k;
+  o->mn_major = l.mn_major;
+  o->z = 1;
+  if (l.direct) {
+    o->p = p;
+    o->ld = l.stride;
+  } else {
+    o->p = copy;
+    o->ld = up8(l.len);
+    const dim3 grid((unsigned)std::min<int64_t>(cdiv(l.len, kEltThreads), 64),
+                    (unsigned)std::min<int64_t>(l.lines, 4096));
+    k_copy_rows<<<grid, kEltThreads, 0, stream>>>(reinterpret_cast<const uint16_t*>(p), l.stride,
+                                                  (int)l.lines, (int)l.len, copy, (int)o->ld);
+    MX_CU(cudaGetLastError());
+  }
+  o->zs = o->ld * l.lines;
+  return TA_OK;
+}
+
+size_t copy_elems(const Lines& l) { return l.direct ? 0 : (size_t)(up8(l.len) * l.lines); }
+
+bool half_type(int dt) { return dt == TA_BF16 || dt == TA_F16; }
+bool any_type(int dt) { return dt == TA_F32 || half_type(dt); }
+
+ta_status check_sizes(int64_t tokens, int64_t fan_in, int64_t fan_out) {
+  if (tokens < 0 || fan_in < 0 || fan_out < 0) return ta_fail(TA_ERR_INVALID, "negative size");
+  if (tokens > kMaxDim || fan_in > kMaxDim || fan_out > kMaxDim)
+    return ta_fail(TA_ERR_UNSUPPORTED, "a size is over 2^31 - 256");
+  return TA_OK;
+}
+
+struct LinearSpace {
+  float* split_ws;
+  uint32_t* split_count;
+  uint16_t *xc, *wc;
+};
+
+ta_status prepare_linear(const ta_linear* op, Lines* x, Lines* w) {
+  if (!op) return ta_fail(TA_ERR_INVALID, "null operator");
+  MX_OK(check_sizes(op->tokens, op->fan_in, op->fan_out));
+  if (!half_type(op->dtype)) return ta_fail(TA_ERR_INVALID, "dtype must be TA_BF16 or TA_F16");
+  if (op->bias_dev && !any_type(op->bias_dtype))
+    return ta_fail(TA_ERR_INVALID, "bias_dtype must be TA_F32, TA_BF16 or TA_F16");
+  if (op->activation < TA_ACT_NONE || op->activation > TA_ACT_SILU)
+    return ta_fail(TA_ERR_INVALID, "unknown activation");
+  if (!lines_of(op->x_dev, op->tokens, op->fan_in, op->x_strides[0], op->x_strides[1], x))
+    return ta_fail(TA_ERR_INVALID, "x needs one unit stride and lines that do not overlap");
+  if (!lines_of(op->w_dev, op->fan_out, op->fan_in, op->w_strides[0], op->w_strides[1], w))
+    return ta_fail(TA_ERR_INVALID, "w needs one unit stride and lines that do not overlap");
+  return TA_OK;
+}
+
+LinearSpace carve_linear(const Lines& x, const Lines& w, Arena* a) {
+  LinearSpace s;
+  s.split_count = a->take<uint32_t>(kSplitUnits);
+  s.split_ws = a->take<float>(kSplitUnits * kSplitTileBytes / 4);
+  s.xc = a->take<uint16_t>(copy_elems(x));
+  s.wc = a->take<uint16_t>(copy_elems(w));
+  return s;
+}
+
+ta_status check_space(const Arena& need, void* ws, size_t bytes, const uint32_t* status) {
+  if (!ws && need.used) return ta_fail(TA_ERR_INVALID, "null workspace");
+  if (bytes < need.used)
+    return ta_fail(TA_ERR_WORKSPACE, "workspace has " + std::to_string(bytes) + " bytes, " +
+                                         std::to_string(need.used) + " are needed");
+  if ((uintptr_t)ws % 256) return ta_fail(TA_ERR_ALIGN, "workspace not 256-byte aligned");
+  if (!status) return ta_fail(TA_ERR_INVALID, "null status word");
+  return TA_OK;
+}
+
+// The products of one linear call: counters are cleared where a launch may split its sums.
+ta_status plain_product(const Product& p, bool bf16, const LinearSpace& s, uint32_t* status,
+                        cudaStream_t stream, bool linear) {
+  const std::vector<Product> ps(1, p);
+  if (choose(ps).splits[0] > 1)
+    MX_CU(cudaMemsetAsync(s.split_count, 0, kSplitUnits * sizeof(uint32_t), stream));
+  if (linear)
+    return run_products<EPI_LINEAR>(ps, bf16, Scalars(), s.split_ws, s.split_count, status, stream);
+  return run_products<EPI_PLAIN>(ps, bf16, Scalars(), s.split_ws, s.split_count, status, stream);
+}
+
+struct GradLines {
+  Lines dz_t, dz_o, x, w;  // dz as tokens x fan_out and as fan_out x tokens; x, w over k
+  bool dw_io = false;      // dw's rows are fan_in
+  bool make_dz = false;
+  int64_t row_parts = 0, ld_dz = 0;
+};
+
+ta_status prepare_grad(const ta_linear_grad* op, GradLines* g) {
+  if (!op) return ta_fail(TA_ERR_INVALID, "null operator");
+  MX_OK(check_sizes(op->tokens, op->fan_in, op->fan_out));
+  if (!half_type(op->dtype)) return ta_fail(TA_ERR_INVALID, "dtype must be TA_BF16 or TA_F16");
+  if (op->db_dev && !any_type(op->bias_dtype))
+    return ta_fail(TA_ERR_INVALID, "bias_dtype must be TA_F32, TA_BF16 or TA_F16");
+  const bool work = op->tokens > 0 && op->fan_out > 0;
+  if (work && !op->dy_dev) return ta_fail(TA_ERR_INVALID, "null dy");
+  if (op->tokens > 1 && op->dy_stride < op->fan_out)
+    return ta_fail(TA_ERR_INVALID, "rows of dy overlap");
+  if (op->dx_dev && op->fan_out > 0 && op->fan_in > 0 && !op->w_dev)
+    return ta_fail(TA_ERR_INVALID, "dx needs w");
+  if (op->dw_dev && op->tokens > 0 && op->fan_in > 0 && !op->x_dev)
+    return ta_fail(TA_ERR_INVALID, "dw needs x");
+  if (op->dx_dev && !lines_of(op->w_dev, op->fan_in, op->fan_out, op->w_strides[1],
+                              op->w_strides[0], &g->w))
+    return ta_fail(TA_ERR_INVALID, "w needs one unit stride and lines that do not overlap");
+  if (op->dw_dev) {
+    if (!lines_of(op->x_dev, op->fan_in, op->tokens, op->x_strides[1], op->x_strides[0], &g->x))
+      return ta_fail(TA_ERR_INVALID, "x needs one unit stride and lines that do not overlap");
+    Lines d;
+    if (!lines_of(op->dw_dev, op->fan_out, op->fan_in, op->dw_strides[0], op->dw_strides[1], &d))
+      return ta_fail(TA_ERR_INVALID, "dw needs one unit stride and lines that do not overlap");
+    g->dw_io = d.mn_major;
+  }
+  const int64_t stride = op->tokens > 1 ? op->dy_stride : up8(op->fan_out);
+  g->make_dz = op->deriv_dev || !aligned16(op->dy_dev) || stride % 8;
+  g->ld_dz = g->make_dz ? up8(op->fan_out) : stride;
+  // rows are split until the blocks of 256 columns fill the SMs some four times
+  if (op->db_dev || g->make_dz)
+    g->row_parts = std::max<int64_t>(
+        1, std::min<int64_t>(cdiv(op->tokens, 16),
+                             cdiv(4 * sm_count(), std::max<int64_t>(1, cdiv(op->fan_out, 256)))));
+  return TA_OK;
+}
+
+struct GradSpace {
+  LinearSpace lin;
+  uint16_t* dz;
+  float* part;
+};
+GradSpace carve_grad(const ta_linear_grad* op, const GradLines& g, Arena* a) {
+  GradSpace s;
+  s.lin = carve_linear(op->dw_dev ? g.x : Lines{false, 0, 0, 0, true},
+                       op->dx_dev ? g.w : Lines{false, 0, 0, 0, true}, a);
+  s.dz = a->take<uint16_t>(g.make_dz ? op->tokens * g.ld_dz : 0);
+  s.part = a->take<float>(op->db_dev ? g.row_parts * op->fan_out : 0);
+  return s;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ta_ortho_workspace_size(const ta_ortho_tensor* tensors, int32_t n_tensors,
+                               const ta_ortho_options* options) {
+  try {
+    ta_fail(TA_OK, "");
+    OrthoPlan plan;
+    if (plan_ortho(tensors, n_tensors, options, &plan) != TA_OK) return 0;
+    Arena a{nullptr};
+    carve_ortho(&plan, &a);
+    return a.used;
+  } catch (const std::exception& e) {
+    ta_fail(TA_ERR_INVALID, e.what());
+    return 0;
+  }
+}
+
+ta_status ta_orthogonalize(const ta_ortho_tensor* tensors, int32_t n_tensors,
+                           const ta_ortho_options* options, void* workspace_dev,
+                           size_t workspace_bytes, uint32_t* status_dev, void* stream) {
+  try {
+    ta_fail(TA_OK, "");
+    OrthoPlan plan;
+    MX_OK(plan_ortho(tensors, n_tensors, options, &plan));
+    if (plan.items == 0) return TA_OK;
+    Arena need{nullptr};
+    carve_ortho(&plan, &need);
+    MX_OK(check_space(need, workspace_dev, workspace_bytes, status_dev));
+    Arena a{reinterpret_cast<uint8_t*>(workspace_dev)};
+    const OrthoSpace sp = carve_ortho(&plan, &a);
+    return run_ortho(tensors, options, plan, sp, status_dev, (cudaStream_t)stream);
+  } catch (const std::exception& e) {
+    return ta_fail(TA_ERR_INVALID, e.what());
+  }
+}
+
+size_t ta_linear_workspace_size(const ta_linear* op) {
+  try {
+    ta_fail(TA_OK, "");
+    Lines x, w;
+    if (prepare_linear(op, &x, &w) != TA_OK) return 0;
+    Arena a{nullptr};
+    carve_linear(x, w, &a);
+    return a.used;
+  } catch (const std::exception& e) {
+    ta_fail(TA_ERR_INVALID, e.what());
+    return 0;
+  }
+}
+
+ta_status ta_linear_forward(const ta_linear* op, void* workspace_dev, size_t workspace_bytes,
+                            uint32_t* status_dev, void* stream_) {
+  try {
+    ta_fail(TA_OK, "");
+    Lines x, w;
+    MX_OK(prepare_linear(op, &x, &w));
+    if (op->tokens == 0 || op->fan_out == 0) return TA_OK;
+    if (!op->y_dev || (op->fan_in > 0 && (!op->x_dev || !op->w_dev)))
+      return ta_fail(TA_ERR_INVALID, "null pointer");
+    if ((op->tokens > 1 && op->y_stride < op->fan_out) ||
+        (op->residual_dev && op->tokens > 1 && op->residual_stride < 0))
+      return ta_fail(TA_ERR_INVALID, "bad row stride");
+    if (op->y_stride > kMaxDim || op->residual_stride > kMaxDim)
+      return ta_fail(TA_ERR_UNSUPPORTED, "a row stride is over 2^31 - 256");
+    if (op->deriv_dev && !aligned16(op->deriv_dev))
+      return ta_fail(TA_ERR_ALIGN, "deriv not 16-byte aligned");
+    Arena need{nullptr};
+    carve_linear(x, w, &need);
+    MX_OK(check_space(need, workspace_dev, workspace_bytes, status_dev));
+    Arena a{reinterpret_cast<uint8_t*>(workspace_dev)};
+    const LinearSpace s = carve_linear(x, w, &a);
+    cudaStream_t stream = (cudaStream_t)stream_;
+    Product p;
+    if (op->fan_in > 0) {
+      MX_OK(operand_of(op->x_dev, op->tokens, op->fan_in, x, s.xc, &p.a, stream));
+      MX_OK(operand_of(op->w_dev, op->fan_out, op->fan_in, w, s.wc, &p.b, stream));
+    }
+    p.M = op->tokens;
+    p.N = op->fan_out;
+    p.ep.za = p.ep.zb = 1;
+    p.ep.dt = (int16_t)op->dtype;
+    p.ep.out = op->y_dev;
+    p.ep.ldo = (int32_t)op->y_stride;
+    p.ep.aux = op->residual_dev;
+    p.ep.ld_aux = (int32_t)op->residual_stride;
+    p.ep.bias = op->bias_dev;
+    p.ep.bias_dt = (int16_t)op->bias_dtype;
+    p.ep.act = (int16_t)op->activation;
+    p.ep.deriv = op->deriv_dev;
+    p.ep.ld_deriv = (int32_t)up8(op->fan_out);
+    return plain_product(p, op->dtype == TA_BF16, s, status_dev, stream, true);
+  } catch (const std::exception& e) {
+    return ta_fail(TA_ERR_INVALID, e.what());
+  }
+}
+
+size_t ta_linear_backward_workspace_size(const ta_linear_grad* op) {
+  try {
+    ta_fail(TA_OK, "");
+    GradLines g;
+    if (prepare_grad(op, &g) != TA_OK) return 0;
+    Arena a{nullptr};
+    carve_grad(op, g, &a);
+    return a.used;
+  } catch (const std::exception& e) {
+    ta_fail(TA_ERR_INVALID, e.what());
+    return 0;
+  }
+}
+
+ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
+                             size_t workspace_bytes, uint32_t* status_dev, void* stream_) {
+  try {
+    ta_fail(TA_OK, "");
+    GradLines g;
+    MX_OK(prepare_grad(op, &g));
+    if (op->deriv_dev && !aligned16(op->deriv_dev))
+      return ta_fail(TA_ERR_ALIGN, "deriv not 16-byte aligned");
+    Arena need{nullptr};
+    carve_grad(op, g, &need);
+    MX_OK(check_space(need, workspace_dev, workspace_bytes, status_dev));
+    Arena a{reinterpret_cast<uint8_t*>(workspace_dev)};
+    const GradSpace s = carve_grad(op, g, &a);
+    cudaStream_t stream = (cudaStream_t)stream_;
+    const int64_t T = op->tokens, I = op->fan_in, O = op->fan_out;
+    const bool bf16 = op->dtype == TA_BF16;
+    const void* dz = g.make_dz ? (const void*)s.dz : op->dy_dev;
+    if (O > 0 && (g.make_dz || op->db_dev)) {
+      const dim3 grid((unsigned)cdiv(O, 256), (unsigned)g.row_parts);
+      k_dz<<<grid, kEltThreads, 0, stream>>>(op->dy_dev, op->dy_stride, op->deriv_dev,
+                                             (int)up8(O), (int)T, (int)O, op->dtype,
+                                             g.make_dz ? s.dz : nullptr, (int)g.ld_dz,
+                                             op->db_dev ? s.part : nullptr);
+      MX_CU(cudaGetLastError());
+      if (op->db_dev) {
+        k_bias_grad<<<(unsigned)cdiv(O, kEltThreads), kEltThreads, 0, stream>>>(
+            s.part, (int)g.row_parts, (int)O, op->db_dev, op->bias_dtype);
+        MX_CU(cudaGetLastError());
+      }
+    }
+    auto dz_operand = [&](bool over_tokens) {  // summed over tokens (dw) or fan_out (dx)
+      Operand o;
+      o.p = dz;
+      o.mn = over_tokens ? O : T;
+      o.k = over_tokens ? T : O;
+      o.mn_major = over_tokens;
+      o.ld = g.ld_dz;
+      o.zs = g.ld_dz * T;
+      return o;
+    };
+    if (op->dx_dev && T > 0 && I > 0) {
+      Product p;
+      if (O > 0) {
+        p.a = dz_operand(false);
+        MX_OK(operand_of(op->w_dev, I, O, g.w, s.lin.wc, &p.b, stream));
+      }
+      p.M = T;
+      p.N = I;
+      p.ep.za = p.ep.zb = 1;
+      p.ep.dt = (int16_t)op->dtype;
+      p.ep.out = op->dx_dev;
+      p.ep.ldo = (int32_t)I;
+      MX_OK(plain_product(p, bf16, s.lin, status_dev, stream, false));
+    }
+    if (op->dw_dev && O > 0 && I > 0) {
+      Product p;
+      Operand xo, zo;
+      if (T > 0) {
+        MX_OK(operand_of(op->x_dev, I, T, g.x, s.lin.xc, &xo, stream));
+        zo = dz_operand(true);
+      }
+      p.a = g.dw_io ? xo : zo;
+      p.b = g.dw_io ? zo : xo;
+      p.M = g.dw_io ? I : O;
+      p.N = g.dw_io ? O : I;
+      const int64_t ldo = op->dw_strides[g.dw_io ? 1 : 0];
+      if (p.M > 1 && ldo > kMaxDim)
+        return ta_fail(TA_ERR_UNSUPPORTED, "a row stride is over 2^31 - 256");
+      p.ep.za = p.ep.zb = 1;
+      p.ep.dt = (int16_t)op->dtype;
+      p.ep.out = op->dw_dev;
+      p.ep.ldo = (int32_t)(p.M > 1 ? ldo : p.N);
+      MX_OK(plain_product(p, bf16, s.lin, status_dev, stream, false));
+    }
+    return TA_OK;
+  } catch (const std::exception& e) {
+    return ta_fail(TA_ERR_INVALID, e.what());
+  }
+}
+
+}  // extern "C"

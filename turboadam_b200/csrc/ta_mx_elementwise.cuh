@@ -1,0 +1,288 @@
+// ta_mx_elementwise.cuh -- the passes around the products of the matrix
+// operators: momentum and norm, scaling into fp16, the activation's gradient
+// with the bias gradient, and operand copies with aligned rows.
+#pragma once
+
+#include "ta_mx_product.cuh"
+
+namespace ta {
+namespace mx {
+
+constexpr int kEltThreads = 256;
+constexpr int kMaxChunks = 256;  // partial sums of one matrix (one per thread of a block)
+
+// ---- table ---------------------------------------------------------------------
+// The items of a list travel as kernel parameters and are written to the workspace by a
+// kernel, so that a call enqueues kernels only and can be captured into a CUDA graph.
+struct ItemSeed {
+  Item it;
+  int32_t first, batch;  // table slots [first, first + batch)
+  int64_t elem_zs;       // elements between the matrices of g, mom and out
+  int64_t x0_zs;         // elements between the scaled matrices
+};
+constexpr int kSeeds = 20;
+struct TableArgs {
+  ItemSeed s[kSeeds];
+  int32_t count;
+  Item* table;
+  Scale* scale;
+  double* partial;
+  uint32_t* zero;  // words to clear
+  int32_t zero_words;
+};
+
+__device__ __forceinline__ const void* offset_dt(const void* p, int64_t elems, int dt) {
+  return p ? reinterpret_cast<const uint8_t*>(p) + elems * (dt == DT_F32 ? 4 : 2) : nullptr;
+}
+
+__global__ void __launch_bounds__(kEltThreads) k_table(const __grid_constant__ TableArgs a) {
+  const int t = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
+  for (int i = t; i < a.zero_words; i += stride) a.zero[i] = 0;
+  for (int k = 0; k < a.count; ++k) {
+    const ItemSeed& s = a.s[k];
+    for (int z = t; z < s.batch; z += stride) {
+      Item it = s.it;
+      it.g = offset_dt(it.g, z * s.elem_zs, it.g_dt);
+      it.mom = const_cast<void*>(offset_dt(it.mom, z * s.elem_zs, it.mom_dt));
+      it.out = const_cast<void*>(offset_dt(it.out, z * s.elem_zs, it.out_dt));
+      it.x0 += z * s.x0_zs;
+      if (it.x0_lo) it.x0_lo += z * s.x0_zs;
+      it.chunk0 += z * it.chunks;
+      it.partial = a.partial + it.chunk0;
+      it.scale = a.scale + s.first + z;
+      a.table[s.first + z] = it;
+    }
+  }
+}
+
+// The item whose chunks hold chunk c.
+__device__ __forceinline__ const Item& find_item(const Item* table, int count, int c) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table[mid].chunk0 <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return table[lo];
+}
+
+// Sum over the block in a fixed order; the result is valid in every thread.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double warp_sum[kEltThreads / 32];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0;
+#pragma unroll
+  for (int i = 0; i < kEltThreads / 32; ++i) s += warp_sum[i];
+  __syncthreads();
+  return s;
+}
+
+struct alignas(16) F8 {
+  float v[8];
+};
+__device__ __forceinline__ F8 load8(const void* p, int64_t i, int dt) {
+  F8 r;
+  if (dt == DT_F32) {
+    const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+    const float4 a = q[0], b = q[1];
+    r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
+    r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+    float2 f;
+    f = unpack16(u.x, dt); r.v[0] = f.x; r.v[1] = f.y;
+    f = unpack16(u.y, dt); r.v[2] = f.x; r.v[3] = f.y;
+    f = unpack16(u.z, dt); r.v[4] = f.x; r.v[5] = f.y;
+    f = unpack16(u.w, dt); r.v[6] = f.x; r.v[7] = f.y;
+  }
+  return r;
+}
+__device__ __forceinline__ void store8(void* p, int64_t i, int dt, const F8& r) {
+  if (dt == DT_F32) {
+    float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
+    q[0] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
+    q[1] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) =
+        make_uint4(pack16(r.v[0], r.v[1], dt), pack16(r.v[2], r.v[3], dt),
+                   pack16(r.v[4], r.v[5], dt), pack16(r.v[6], r.v[7], dt));
+  }
+}
+// A momentum kept in 16 bits enters the update as it is stored.
+__device__ __forceinline__ float as_stored(float v, int dt) {
+  if (dt == DT_BF16) return __bfloat162float(__float2bfloat16_rn(v));
+  if (dt == DT_F16) return __half2float(__float2half_rn(v));
+  return v;
+}
+__device__ __forceinline__ float direction(float g, float m, float mu, bool nesterov) {
+  return nesterov ? fmaf(mu, m, (1.f - mu) * g) : m;
+}
+__device__ __forceinline__ bool item_vec(const Item& it) {
+  return it.n % 8 == 0 && (((uintptr_t)it.g | (uintptr_t)it.mom) & 15) == 0;
+}
+
+// Momentum m <- mu m + (1 - mu) g, and a chunk's sum of squares of the update direction. Bound
+// by the bytes of g and m. The squares are summed in 64 bits: gradients whose squares leave
+// fp32's range keep their norm.
+__global__ void __launch_bounds__(kEltThreads)
+    k_norm(const Item* table, int count, float mu, int nesterov) {
+  const Item& it = find_item(table, count, blockIdx.x);
+  const int chunk = blockIdx.x - it.chunk0;
+  const int64_t e0 = chunk * it.chunk_elems, e1 = min(it.n, e0 + it.chunk_elems);
+  double sum = 0;
+  if (item_vec(it)) {
+    for (int64_t i = e0 + threadIdx.x * 8; i < e1; i += kEltThreads * 8) {
+      F8 g = load8(it.g, i, it.g_dt);
+      if (it.mom) {
+        F8 m = load8(it.mom, i, it.mom_dt);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m.v[k] = as_stored(fmaf(mu, m.v[k], (1.f - mu) * g.v[k]), it.mom_dt);
+          g.v[k] = direction(g.v[k], m.v[k], mu, nesterov);
+        }
+        store8(it.mom, i, it.mom_dt, m);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum = fma((double)g.v[k], (double)g.v[k], sum);
+    }
+  } else {
+    for (int64_t i = e0 + threadIdx.x; i < e1; i += kEltThreads) {
+      float u = load_as_float(it.g, i, it.g_dt);
+      if (it.mom) {
+        const float m = as_stored(fmaf(mu, load_as_float(it.mom, i, it.mom_dt), (1.f - mu) * u),
+                                  it.mom_dt);
+        store_from_float(it.mom, i, it.mom_dt, m);
+        u = direction(u, m, mu, nesterov);
+      }
+      sum = fma((double)u, (double)u, sum);
+    }
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) it.partial[chunk] = sum;
+}
+
+// The update direction scaled by a power of two into fp16: its Frobenius norm lands in
+// [2^13, 2^14), so that no element overflows and one 2^-38 of the norm still has a code. The
+// scaling is exact; the division by the norm (plus eps) follows in 32 bits behind the products
+// (Scale::unit). A 16-bit input enters without any rounding, a 32-bit one as a pair of fp16
+// numbers where x0_lo is given (22 bits) and rounded once otherwise.
+__global__ void __launch_bounds__(kEltThreads)
+    k_scale(const Item* table, int count, float mu, int nesterov, double eps) {
+  const Item& it = find_item(table, count, blockIdx.x);
+  const int chunk = blockIdx.x - it.chunk0;
+  const double norm = sqrt(block_sum((int)threadIdx.x < it.chunks ? it.partial[threadIdx.x] : 0.0));
+  float pow2 = 1.f, unit = 0.f;
+  if (!(norm <= 1.7e308)) {
+    unit = __int_as_float(0x7fc00000);
+  } else if (norm > 0) {
+    pow2 = ldexpf(1.f, max(-126, min(120, 13 - ilogb(norm))));
+    unit = (float)(1.0 / ((norm + eps) * (double)pow2));
+  }
+  if (chunk == 0 && threadIdx.x == 0) *it.scale = Scale{pow2, unit};
+  const int64_t e0 = chunk * it.chunk_elems, e1 = min(it.n, e0 + it.chunk_elems);
+  if (item_vec(it) && it.cols == it.ld) {
+    for (int64_t i = e0 + threadIdx.x * 8; i < e1; i += kEltThreads * 8) {
+      F8 g = load8(it.g, i, it.g_dt);
+      if (it.mom) {
+        const F8 m = load8(it.mom, i, it.mom_dt);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g.v[k] = direction(g.v[k], m.v[k], mu, nesterov);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g.v[k] *= pow2;
+      store8(it.x0, i, DT_F16, g);
+      if (it.x0_lo) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g.v[k] -= __half2float(__float2half_rn(g.v[k]));
+        store8(it.x0_lo, i, DT_F16, g);
+      }
+    }
+  } else {
+    for (int64_t i = e0 + threadIdx.x; i < e1; i += kEltThreads) {
+      float u = load_as_float(it.g, i, it.g_dt);
+      if (it.mom) u = direction(u, load_as_float(it.mom, i, it.mom_dt), mu, nesterov);
+      u *= pow2;
+      const int64_t r = it.n <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)it.cols)
+                                           : i / it.cols;
+      const int64_t at = r * it.ld + (i - r * it.cols);
+      const __half hi = __float2half_rn(u);
+      it.x0[at] = hi;
+      if (it.x0_lo) it.x0_lo[at] = __float2half_rn(u - __half2float(hi));
+    }
+  }
+}
+
+// ---- operand copies --------------------------------------------------------------
+// rows x cols 16-bit elements into rows of ld elements (TMA reads rows that start on 16 bytes).
+__global__ void __launch_bounds__(kEltThreads)
+    k_copy_rows(const uint16_t* src, int64_t stride, int rows, int cols, uint16_t* dst, int ld) {
+  for (int r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int c = blockIdx.x * kEltThreads + threadIdx.x; c < cols; c += gridDim.x * kEltThreads)
+      dst[(int64_t)r * ld + c] = src[(int64_t)r * stride + c];
+}
+
+// ---- gradient of the activation, and of the bias -----------------------------------
+// dz = dy act'(z), rounded to the operand type for the two products that read it; the bias
+// gradient sums the unrounded dz. Block (x, y) takes 256 columns and the y-th range of rows; its
+// column sums go to part[y], which k_bias_grad adds in order.
+__global__ void __launch_bounds__(kEltThreads)
+    k_dz(const void* dy, int64_t dy_stride, const int16_t* deriv, int ld_deriv, int rows, int cols,
+         int dt, uint16_t* dz, int ld_dz, float* part) {
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int c0 = blockIdx.x * 256 + lane * 8;
+  const int r0 = (int)((int64_t)rows * blockIdx.y / gridDim.y);
+  const int r1 = (int)((int64_t)rows * (blockIdx.y + 1) / gridDim.y);
+  const bool vec = c0 + 8 <= cols && dy_stride % 8 == 0 && ((uintptr_t)dy & 15) == 0;
+  float sum[8] = {};
+  for (int r = r0 + sub; r < r1; r += 8) {
+    F8 g;
+    const int64_t at = (int64_t)r * dy_stride + c0;
+    if (vec) {
+      g = load8(dy, at, dt);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g.v[k] = c0 + k < cols ? load_as_float(dy, at + k, dt) : 0.f;
+    }
+    if (deriv && c0 < cols) {  // rows of ld_deriv (a multiple of 8) codes
+      const uint4 u = *reinterpret_cast<const uint4*>(deriv + (int64_t)r * ld_deriv + c0);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c0 + k < cols) g.v[k] *= decode_deriv((int16_t)(w[k >> 1] >> (16 * (k & 1))));
+    }
+    if (dz && c0 < cols) {
+      if (c0 + 8 <= cols) {
+        store8(dz, (int64_t)r * ld_dz + c0, dt, g);
+      } else {
+        for (int k = 0; c0 + k < cols; ++k) store_from_float(dz, (int64_t)r * ld_dz + c0 + k, dt, g.v[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] += g.v[k];
+  }
+  if (part) {
+    __shared__ float s[8][256];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[sub][lane * 8 + k] = sum[k];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    float t = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += s[i][threadIdx.x];
+    if (c < cols) part[(int64_t)blockIdx.y * cols + c] = t;
+  }
+}
+__global__ void __launch_bounds__(kEltThreads)
+    k_bias_grad(const float* part, int parts, int cols, void* db, int dt) {
+  const int c = blockIdx.x * kEltThreads + threadIdx.x;
+  if (c >= cols) return;
+  float t = 0;
+  for (int i = 0; i < parts; ++i) t += part[(int64_t)i * cols + c];
+  store_from_float(db, c, dt, t);
+}
+
+}  // namespace mx
+}  // namespace ta

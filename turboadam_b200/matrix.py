@@ -1,0 +1,291 @@
+"""Matrix operators beside the packed optimizer step (include/turboadam_b200_matrix.h).
+
+* :func:`linear_act` -- a linear layer with bias, activation and residual in
+  its product's epilogue, and its gradients;
+* :func:`orthogonalize` -- the Newton-Schulz iteration of the Muon optimizer;
+* :class:`turboadam_b200.Muon` (muon.py) -- the optimizer step built on it.
+
+Like the optimizer, they run on CUDA (sm_100a) tensors only; there is no CPU
+fallback. None has a counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+# the quintic of the Muon optimizer, tuned for slope at zero
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+NS_STEPS = 5
+NS_EPS = 1e-7
+
+_DTYPES = {torch.float32: _lib.TA_F32, torch.bfloat16: _lib.TA_BF16, torch.float16: _lib.TA_F16}
+_HALF = (torch.bfloat16, torch.float16)
+_ACTIVATIONS = {None: _lib.TA_ACT_NONE, "none": _lib.TA_ACT_NONE, "relu": _lib.TA_ACT_RELU,
+                "gelu": _lib.TA_ACT_GELU, "gelu_tanh": _lib.TA_ACT_GELU_TANH,
+                "silu": _lib.TA_ACT_SILU}
+
+_status = {}  # device index -> int32 [1], OR-ed into by every call on that device
+
+
+def status_word(device: torch.device) -> torch.Tensor:
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    st = _status.get(idx)
+    if st is None:
+        st = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        torch.cuda.synchronize(st.device)  # zeroed before any stream uses it
+        _status[idx] = st
+    return st
+
+
+def read_status(clear: bool = True) -> int:
+    """Device status bits of the matrix operators since the last read, over
+    all devices (TA_STATUS_WAIT_TIMEOUT: a bounded wait ran out and that
+    call's results are void). Synchronises."""
+    lib = _lib.load()
+    out = 0
+    for idx, st in _status.items():
+        v = ctypes.c_uint32(0)
+        with torch.cuda.device(idx):
+            torch.cuda.synchronize(idx)
+            _lib.check(lib.ta_read_status(st.data_ptr(), int(clear), ctypes.byref(v),
+                                          _lib.stream_ptr(idx)), "ta_read_status")
+        out |= v.value
+    return out
+
+
+def check_coefficients(coefficients, steps: int):
+    """One (a, b, c), or one per step, as a flat list of 3 * steps floats."""
+    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= 32:
+        raise ValueError(f"steps must be a whole number from 1 to 32, got {steps}")
+    rows = list(coefficients)
+    if len(rows) == 3 and not any(hasattr(r, "__len__") for r in rows):
+        rows = [rows] * int(steps)
+    if len(rows) != steps or any(not hasattr(r, "__len__") or len(r) != 3 for r in rows):
+        raise ValueError("coefficients must be one (a, b, c) or one (a, b, c) per step")
+    return [float(v) for r in rows for v in r]
+
+
+def ortho_options(coefficients, steps, eps, momentum=0.0, nesterov=False):
+    """The ABI options, and the host array they point at."""
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    flat = check_coefficients(coefficients, steps)
+    arr = (ctypes.c_double * len(flat))(*flat)
+    return _lib.TaOrthoOptions(ctypes.cast(arr, ctypes.c_void_p), int(steps), int(nesterov),
+                               float(eps), float(momentum)), arr
+
+
+def run_ortho(table, n, options, dev):
+    """One ta_orthogonalize call on the current stream of ``dev``."""
+    lib = _lib.load()
+    need = lib.ta_ortho_workspace_size(table, n, ctypes.byref(options))
+    if need == 0 and lib.ta_last_error():
+        raise _lib.TurboAdamBackendError(
+            f"ta_ortho_workspace_size failed: {lib.ta_last_error().decode(errors='replace')}")
+    with torch.cuda.device(dev):
+        # allocated on the current stream: reused only for work ordered after this call
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        rc = lib.ta_orthogonalize(table, n, ctypes.byref(options), ws.data_ptr(), ws.numel(),
+                                  status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc, "ta_orthogonalize")
+
+
+@torch.no_grad()
+def orthogonalize(x: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFICIENTS,
+                  eps: float = NS_EPS, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of a matrix or a stack of matrices.
+
+    With X = x / (|x|_F + eps) and, ``steps`` times, A = X X^T (X^T X for a
+    tall matrix), X <- (a I + b A + c A^2) X; returns X in ``dtype``.
+    ``coefficients`` is one (a, b, c), by default the Muon quintic, or one per
+    step. x: float32, bfloat16 or float16, [..., rows, cols].
+
+    The products take fp16 operands and fp32 sums. A 16-bit x enters
+    unrounded, a 32-bit one as a pair of fp16 numbers; the result is within
+    about 1e-3 of the exact iteration (2-norm), so float32 outputs carry about
+    ten good bits. A zero matrix gives zero; a matrix with a NaN or an
+    infinity gives NaN throughout. Not differentiable.
+    """
+    _lib.require_cuda(x)
+    if x.dim() < 2:
+        raise ValueError(f"orthogonalize takes matrices, got {x.dim()} dimension(s)")
+    if x.dtype not in _DTYPES or dtype not in _DTYPES:
+        raise NotImplementedError(f"orthogonalize: dtypes {x.dtype} -> {dtype} (float32, bfloat16 "
+                                  "and float16 are built)")
+    options, keep = ortho_options(coefficients, steps, eps)
+    src = x.contiguous()
+    out = torch.empty(x.shape, dtype=dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    rows, cols = x.shape[-2:]
+    table = (_lib.TaOrthoTensor * 1)()
+    t = table[0]
+    t.in_dev, t.out_dev = src.data_ptr(), out.data_ptr()
+    t.batch, t.rows, t.cols = x.numel() // (rows * cols), rows, cols
+    t.in_dtype, t.out_dtype = _DTYPES[x.dtype], _DTYPES[dtype]
+    t.flags = _lib.TA_ORTHO_PAIR
+    run_ortho(table, 1, options, x.device)
+    return out
+
+
+def _two_strides(t: torch.Tensor) -> torch.Tensor:
+    """A matrix the products can read: one unit stride, lines that do not overlap."""
+    (r, c), (sr, sc) = t.shape, t.stride()
+    if (c <= 1 or sc == 1) and (r <= 1 or sr >= c):
+        return t
+    if (r <= 1 or sr == 1) and (c <= 1 or sc >= r):
+        return t
+    return t.contiguous()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix with unit column stride and rows that do not overlap."""
+    (r, c), (sr, sc) = t.shape, t.stride()
+    return t if (c <= 1 or sc == 1) and (r <= 1 or sr >= c) else t.contiguous()
+
+
+def _strides(t):
+    return (ctypes.c_int64 * 2)(*t.stride())
+
+
+def _call_linear(fn_size, fn, what, op, dev):
+    lib = _lib.load()
+    need = fn_size(ctypes.byref(op))
+    if need == 0 and lib.ta_last_error():
+        raise _lib.TurboAdamBackendError(
+            f"{what} failed: {lib.ta_last_error().decode(errors='replace')}")
+    with torch.cuda.device(dev):
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        rc = fn(ctypes.byref(op), ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(),
+                _lib.stream_ptr(dev))
+    _lib.check(rc, what)
+
+
+def _forward(x, w, bias, act, residual, need_deriv):
+    lib = _lib.load()
+    x, w = _two_strides(x), _two_strides(w)
+    tokens, fan_in, fan_out = x.shape[0], x.shape[1], w.shape[0]
+    y = torch.empty(tokens, fan_out, dtype=x.dtype, device=x.device)
+    deriv = None
+    if need_deriv:
+        deriv = torch.empty(tokens, (fan_out + 7) // 8 * 8, dtype=torch.int16, device=x.device)
+    op = _lib.TaLinear()
+    op.x_dev, op.w_dev, op.y_dev = x.data_ptr(), w.data_ptr(), y.data_ptr()
+    op.tokens, op.fan_in, op.fan_out = tokens, fan_in, fan_out
+    op.x_strides, op.w_strides = _strides(x), _strides(w)
+    op.y_stride = max(fan_out, 1)
+    op.dtype, op.activation = _DTYPES[x.dtype], act
+    if bias is not None:
+        bias = bias.contiguous()
+        op.bias_dev, op.bias_dtype = bias.data_ptr(), _DTYPES[bias.dtype]
+    if residual is not None:
+        residual = _rows(residual)
+        op.residual_dev, op.residual_stride = residual.data_ptr(), residual.stride(0)
+    if deriv is not None:
+        op.deriv_dev = deriv.data_ptr()
+    if y.numel():
+        _call_linear(lib.ta_linear_workspace_size, lib.ta_linear_forward, "ta_linear_forward", op,
+                     x.device)
+    return y, deriv
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, act):
+        # the derivative is needed by every gradient but the residual's
+        need = act != _lib.TA_ACT_NONE and any(ctx.needs_input_grad[:3])
+        y, deriv = _forward(x, w, bias, act, residual, need)
+        ctx.act = act
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None,
+                              w if ctx.needs_input_grad[0] else None, deriv)
+        ctx.dims = (x.shape[0], x.shape[1], w.shape[0])
+        # the weight's gradient is laid out as the weight: input by output if its rows are
+        ctx.io = w.stride(0) == 1 and w.stride(1) != 1
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, deriv = ctx.saved_tensors
+        tokens, fan_in, fan_out = ctx.dims
+        nx, nw, nb, nr, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if nx or nw or nb:
+            lib = _lib.load()
+            g = _rows(dy)
+            op = _lib.TaLinearGrad()
+            op.dy_dev, op.dy_stride = g.data_ptr(), max(g.stride(0), fan_out)
+            op.tokens, op.fan_in, op.fan_out = tokens, fan_in, fan_out
+            op.dtype = _DTYPES[dy.dtype]
+            if deriv is not None:
+                op.deriv_dev = deriv.data_ptr()
+            if nx:
+                w = _two_strides(w)
+                op.w_dev, op.w_strides = w.data_ptr(), _strides(w)
+                dx = torch.empty(tokens, fan_in, dtype=dy.dtype, device=dy.device)
+                op.dx_dev = dx.data_ptr()
+            if nw:
+                x = _two_strides(x)
+                op.x_dev, op.x_strides = x.data_ptr(), _strides(x)
+                if ctx.io:
+                    dw = torch.empty(fan_in, fan_out, dtype=dy.dtype, device=dy.device).t()
+                else:
+                    dw = torch.empty(fan_out, fan_in, dtype=dy.dtype, device=dy.device)
+                op.dw_dev, op.dw_strides = dw.data_ptr(), _strides(dw)
+            if nb:
+                db = torch.empty(fan_out, dtype=ctx.bias_dtype, device=dy.device)
+                op.db_dev, op.bias_dtype = db.data_ptr(), _DTYPES[db.dtype]
+            _call_linear(lib.ta_linear_backward_workspace_size, lib.ta_linear_backward,
+                         "ta_linear_backward", op, dy.device)
+        return dx, dw, db, dy if nr else None, None
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+               activation: str | None = None,
+               residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``activation(x @ weight.T + bias) + residual`` as one product.
+
+    x: [..., fan_in], weight: [fan_out, fan_in] (a transposed view of an
+    input-by-output weight is read as it lies), bias: [fan_out], residual:
+    [..., fan_out]; activation: None, "relu", "gelu", "gelu_tanh" or "silu".
+    x, weight and residual are all bfloat16 or all float16; the bias may also
+    be float32. Sums, bias, activation and residual are in fp32 and rounded
+    once.
+
+    Differentiable once in x, weight, bias and residual. For the backward pass
+    the activation's derivative is kept (16-bit fixed point, steps of 2^-14);
+    dz = dy * derivative is rounded once to the operand type for the two
+    products that read it. A weight's gradient has the weight's layout.
+    """
+    _lib.require_cuda(x)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(k for k in _ACTIVATIONS if k)} or "
+                         f"None, got {activation!r}")
+    if x.dtype not in _HALF:
+        raise NotImplementedError(f"linear_act is built for bfloat16 and float16, got {x.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match: "
+                         "[..., fan_in] and [fan_out, fan_in] are wanted")
+    fan_out = weight.shape[0]
+    shape = (*x.shape[:-1], fan_out)
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+        if t.dtype != x.dtype and not (name == "bias" and t.dtype == torch.float32):
+            raise ValueError(f"{name} has dtype {t.dtype}, x has {x.dtype}")
+    if bias is not None and tuple(bias.shape) != (fan_out,):
+        raise ValueError(f"bias has shape {tuple(bias.shape)}, wanted {(fan_out,)}")
+    if residual is not None and tuple(residual.shape) != shape:
+        raise ValueError(f"residual has shape {tuple(residual.shape)}, wanted {shape}")
+    tokens = 1
+    for d in x.shape[:-1]:
+        tokens *= d
+    x2 = x.reshape(tokens, x.shape[-1])
+    r2 = None if residual is None else residual.reshape(tokens, fan_out)
+    return _LinearAct.apply(x2, weight, bias, r2, _ACTIVATIONS[activation]).reshape(shape)
