@@ -95,14 +95,15 @@ struct Operand {
   bool mn_major = false;
 };
 
-ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16) {
+// box_mn: rows (or columns) of the output one copy brings; an mn-major operand comes in chunks of 64.
+ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn) {
   EncodeFn fn = encode_fn();
   if (!fn) return ta_fail(TA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const int64_t inner = o.mn_major ? o.mn : o.k, lines = o.mn_major ? o.k : o.mn;
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)lines, (cuuint64_t)o.z};
   cuuint64_t strides[2] = {(cuuint64_t)(o.ld * 2),
                            (cuuint64_t)(std::max<int64_t>(o.zs, o.ld) * 2)};
-  cuuint32_t box[3] = {64, (cuuint32_t)(o.mn_major ? kDepth : kRows), 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)(o.mn_major ? kDepth : box_mn), 1};
   cuuint32_t step[3] = {1, 1, 1};
   CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                   const_cast<void*>(o.p), dims, strides, box, step,
@@ -124,70 +125,104 @@ struct Product {
   Product() { memset(&ep, 0, sizeof(ep)); }
 };
 
-int64_t tiles_of(const Product& p, int cg, int* tm = nullptr, int* tn = nullptr) {
-  const int64_t side = 128 * cg, m = cdiv(p.M, side), n = cdiv(p.N, side);
-  if (tm) *tm = (int)m;
-  if (tn) *tn = (int)n;
-  return p.sym ? m * (m + 1) / 2 : m * n;
-}
 int64_t blocks_of(const Product& p) { return cdiv(p.a.k, kDepth) * p.parts; }
 
+int64_t tiles_of(const Product& p, int cols) {
+  const int64_t m = cdiv(p.M, kTileRows), n = cdiv(p.N, cols);
+  if (!p.sym) return m * n;
+  int64_t t = 0;
+  for (int64_t i = 0; i < m; ++i) t += n - sym_first((int)i, cols);
+  return t;
+}
+
 struct Shape {
-  int cg = 1;
+  int cols = 256;
   std::vector<int> splits;
 };
 
-constexpr int64_t kSplitUnits = 296;  // room for the split tiles of one launch
-constexpr size_t kSplitTileBytes = (size_t)kRows * 128 * 4;
+// room for the split tiles of one launch
+constexpr int64_t kSplitTiles = 592;                    // counters: one per CTA tile
+constexpr int64_t kSplitFloats = 320ll * kRows * 256;   // partial sums
 
-// Tile and splits of a launch. The large tile runs at the tensor pipe's rate and the small one
-// at about 0.85 of it (shared-memory bandwidth), so the small one is for lists whose large tiles
-// would leave pairs of SMs idle: the lower estimate of (rounds of tiles) x (time of a tile) wins.
-// Where even the small tiles do not fill the SMs, sums of 8 or more k blocks are split until
-// they do.
-Shape choose(const std::vector<Product>& ps) {
-  const int sms = sm_count();
-  int64_t u1 = 0, u2 = 0, w1 = 0, w2 = 0, longest = 0;
-  for (const Product& p : ps) {
-    const int64_t kb = std::max<int64_t>(1, blocks_of(p));
-    const int64_t t1 = tiles_of(p, 1) * p.batch, t2 = tiles_of(p, 2) * p.batch;
-    u1 += t1;
-    u2 += t2;
-    w1 += t1 * kb;
-    w2 += t2 * kb;
-    longest = std::max(longest, kb);
-  }
-  Shape s;
-  s.splits.assign(ps.size(), 1);
-  if (u1 == 0) return s;
-  const double rounds1 = (double)cdiv(u1, sms), rounds2 = (double)cdiv(u2, sms / 2);
-  const double time2 = std::max(rounds2 * (double)w2 / (double)u2, (double)longest) * 2.0;
-  const bool split = u1 * 2 <= sms && longest >= 16;
-  const double time1 =
-      (split ? (double)w1 / sms + 8 : std::max(rounds1 * (double)w1 / (double)u1, (double)longest)) *
-      1.18;
-  if (time2 <= time1) {
-    s.cg = 2;
-    return s;
-  }
-  if (split) {
-    const double ideal = std::max(8.0, (double)w1 / sms);
-    int64_t units = 0;
-    for (size_t i = 0; i < ps.size(); ++i) {
-      const int64_t kb = blocks_of(ps[i]);
-      s.splits[i] = (int)std::max<int64_t>(1, std::min<int64_t>(32, (int64_t)(kb / ideal)));
-      if (s.splits[i] > 1) units += tiles_of(ps[i], 1) * ps[i].batch * s.splits[i];
-    }
-    if (units > kSplitUnits) s.splits.assign(ps.size(), 1);
-  }
-  return s;
+// SM cycles of a pair's tile of `cols` columns: per block of 64 k's the tensor pipe needs 2 cols
+// and shared memory 256 + cols; each gets in the other's way by about half of the smaller. The
+// epilogue of a single-accumulator tile (cols > 256) is not hidden; a tile costs about 1500 cycles
+// to begin and end.
+double tile_cycles(double kblocks, int cols) {
+  const double mma = 2.0 * cols, mem = 256.0 + cols;
+  const double loop = kblocks * (std::max(mma, mem) + 0.5 * std::min(mma, mem) * (mem > 0.9 * mma));
+  const double epilogue = 1000.0 + 12.0 * cols;
+  return cols > 256 ? loop + epilogue + 500 : std::max(loop, epilogue) + 500;
 }
 
-// Shared-memory limit and resident CTAs (or CTA pairs) of an instance, found once per device. A
-// die's SM count need not divide into pairs, so the pairs that fit are asked for: a pair that had
-// to wait for another to finish would double the time of a persistent launch.
-template <int CG, int EPI>
-ta_status workers_of(int* workers) {
+// Tile width and splits of a launch: the lowest estimate of (rounds of tiles) x (time of a tile)
+// over the widths the operands' layouts allow. Wide tiles use the tensor pipe best, narrow ones
+// give every pair of SMs a share of a small result. Where even the narrow ones do not, long sums
+// are split: the partial tiles cost about 3000 cycles and a pass over them per split.
+Shape choose(const std::vector<Product>& ps, int pairs) {
+  bool b_mn = false;
+  for (const Product& p : ps) b_mn = b_mn || p.b.mn_major;
+  static const int kAny[] = {512, 448, 384, 320, 256, 192, 128, 64}, kChunked[] = {512, 256, 128};
+  const int* widths = b_mn ? kChunked : kAny;
+  const int n_widths = b_mn ? 3 : 8;
+  Shape best;
+  best.splits.assign(ps.size(), 1);
+  double best_time = 1e300;
+  for (int k = 0; k < n_widths; ++k) {
+    const int cols = widths[k];
+    int64_t units = 0;
+    double work = 0, longest = 0;
+    for (const Product& p : ps) {
+      const int64_t t = tiles_of(p, cols) * p.batch;
+      const double c = tile_cycles((double)blocks_of(p), cols);
+      units += t;
+      work += (double)t * c;
+      longest = std::max(longest, c);
+    }
+    if (units == 0) return best;
+    double time = ps.size() == 1 ? (double)cdiv(units, pairs) * longest
+                                 : std::max(longest, work / pairs + 0.5 * longest);
+    std::vector<int> splits(ps.size(), 1);
+    if (units * 2 <= pairs) {
+      // so many that each pair gets one split of the longest sums
+      double split_work = 0, split_longest = 0;
+      int64_t tiles = 0, floats = 0, split_units = 0;
+      const double ideal = work / pairs;
+      for (size_t i = 0; i < ps.size(); ++i) {
+        const int64_t kb = blocks_of(ps[i]), t = tiles_of(ps[i], cols) * ps[i].batch;
+        const double c = tile_cycles((double)kb, cols);
+        splits[i] = (int)std::max<int64_t>(
+            1, std::min<int64_t>({kb / 2, (int64_t)(c / std::max(ideal, 1.0)), (int64_t)16}));
+        const double one = tile_cycles((double)cdiv(kb, splits[i]), cols) +
+                           (splits[i] > 1 ? 3000.0 + splits[i] * 2.5 * cols : 0.0);
+        split_units += t * splits[i];
+        split_work += (double)t * splits[i] * one;
+        split_longest = std::max(split_longest, one);
+        if (splits[i] > 1) {
+          tiles += 2 * t;
+          floats += 2 * t * splits[i] * kRows * cols;
+        }
+      }
+      const double split_time = ps.size() == 1
+                                    ? (double)cdiv(split_units, pairs) * split_longest
+                                    : std::max(split_longest, split_work / pairs);
+      if (split_time < time && tiles <= kSplitTiles && floats <= kSplitFloats) time = split_time;
+      else splits.assign(ps.size(), 1);
+    }
+    if (time < best_time) {
+      best_time = time;
+      best.cols = cols;
+      best.splits = splits;
+    }
+  }
+  return best;
+}
+
+// Shared-memory limit and resident pairs of an instance, found once per device. A die's SM count
+// need not divide into pairs, so the pairs that fit are asked for: one that had to wait for
+// another to finish would double the time of a persistent launch.
+template <int EPI, int DT>
+ta_status pairs_of(int* pairs) {
   constexpr int kMaxDevices = 64;
   static std::mutex m;
   static int found[kMaxDevices] = {};
@@ -196,48 +231,32 @@ ta_status workers_of(int* workers) {
   if (dev >= kMaxDevices) return ta_fail(TA_ERR_UNSUPPORTED, "device index over 63");
   std::lock_guard<std::mutex> lock(m);
   if (!found[dev]) {
-    MX_CU(cudaFuncSetAttribute(k_product<CG, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    MX_CU(cudaFuncSetAttribute(k_product<EPI, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)kProductSmem));
-    int n = sm_count();
-    if (CG == 2) {
-      cudaLaunchConfig_t cfg = {};
-      cudaLaunchAttribute attr;
-      attr.id = cudaLaunchAttributeClusterDimension;
-      attr.val.clusterDim.x = 2;
-      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-      cfg.gridDim = dim3((unsigned)(n / 2 * 2));
-      cfg.blockDim = dim3(kThreads);
-      cfg.dynamicSmemBytes = kProductSmem;
-      cfg.attrs = &attr;
-      cfg.numAttrs = 1;
-      MX_CU(cudaOccupancyMaxActiveClusters(&n, k_product<CG, EPI>, &cfg));
-    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(sm_count() / 2 * 2));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kProductSmem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    MX_CU(cudaOccupancyMaxActiveClusters(&n, k_product<EPI, DT>, &cfg));
     if (n < 1) return ta_fail(TA_ERR_CUDA, "the product kernel does not fit this device");
     found[dev] = n;
   }
-  *workers = found[dev];
+  *pairs = found[dev];
   return TA_OK;
 }
 
-template <int CG, int EPI>
-ta_status launch_product(const ProductArgs& g, cudaStream_t stream) {
-  int workers = 0;
-  MX_OK((workers_of<CG, EPI>(&workers)));
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(g.units, workers)));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kProductSmem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 0;
-  if (CG == 2) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  }
-  MX_CU(cudaLaunchKernelEx(&cfg, k_product<CG, EPI>, g));
+template <int EPI, int DT>
+ta_status launch_product(const ProductArgs& g, int pairs, cudaStream_t stream) {
+  const unsigned grid = 2u * (unsigned)std::min<int64_t>(g.units, pairs);
+  k_product<EPI, DT><<<grid, kThreads, kProductSmem, stream>>>(g);
+  MX_CU(cudaGetLastError());
   return TA_OK;
 }
 
@@ -246,16 +265,19 @@ struct Scalars {
   int unit_pow = 0;
 };
 
-// split_ws / split_count: room for kSplitUnits tiles and counters (zero).
-template <int EPI>
+// split_ws / split_count: kSplitFloats and kSplitTiles of them; the counters are zero, or `clear`ed
+// here where a launch splits its sums.
+template <int EPI, int DT = DT_F16>
 ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars& sc,
-                       float* split_ws, uint32_t* split_count, uint32_t* status,
+                       float* split_ws, uint32_t* split_count, bool clear, uint32_t* status,
                        cudaStream_t stream) {
   for (size_t lo = 0; lo < all.size(); lo += kMaxProblems) {
     const std::vector<Product> ps(all.begin() + lo,
                                   all.begin() + std::min(all.size(), lo + kMaxProblems));
     MX_OK(bind_device());
-    Shape shape = choose(ps);
+    int pairs = 0;
+    MX_OK((pairs_of<EPI, DT>(&pairs)));
+    const Shape shape = choose(ps, pairs);
     ProductArgs g;
     memset(&g, 0, sizeof(g));
     g.count = (int)ps.size();
@@ -266,20 +288,28 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
     g.c2 = sc.c2;
     g.unit_pow = sc.unit_pow;
     g.status = status;
-    int64_t units = 0, split_units = 0, split_tiles = 0;
+    g.cols = shape.cols;
+    g.halves = shape.cols > 256 ? 2 : 1;
+    g.half = shape.cols / g.halves;
+    g.buffers = shape.cols > 256 ? 1 : 2;
+    g.stages = (int)std::min<size_t>(
+        kMaxStages, kOperandSpace / (size_t)(kTileABytes + shape.cols * kDepth));
+    int64_t units = 0, split_floats = 0, split_tiles = 0;
     for (size_t i = 0; i < ps.size(); ++i) {
       const Product& p = ps[i];
       Problem& P = g.p[i];
       P = p.ep;
       if (p.a.k > 0) {
-        MX_OK(make_map(&P.ta, p.a, bf16));
-        MX_OK(make_map(&P.tb, p.b, bf16));
+        MX_OK(make_map(&P.ta, p.a, bf16, kRows));
+        MX_OK(make_map(&P.tb, p.b, bf16, g.half / 2));
       }
       P.M = (int32_t)p.M;
       P.N = (int32_t)p.N;
       P.kblocks = (int32_t)cdiv(p.a.k, kDepth);
       P.parts = p.parts;
-      P.tiles = (int32_t)tiles_of(p, shape.cg, &P.tiles_m, &P.tiles_n);
+      P.tiles_m = (int32_t)cdiv(p.M, kTileRows);
+      P.tiles_n = (int32_t)cdiv(p.N, shape.cols);
+      P.tiles = (int32_t)tiles_of(p, shape.cols);
       P.first = (int32_t)units;
       P.batch = (int32_t)p.batch;
       P.splits = shape.splits[i];
@@ -288,18 +318,19 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
       P.sym = p.sym;
       const int64_t tiles = (int64_t)P.tiles * p.batch;
       if (P.splits > 1) {
-        P.split_ws = split_ws + split_units * (kSplitTileBytes / 4);
+        P.split_ws = split_ws + split_floats;
         P.split_count = split_count + split_tiles;
-        split_units += tiles * P.splits;
-        split_tiles += tiles;
+        split_floats += 2 * tiles * P.splits * kRows * shape.cols;
+        split_tiles += 2 * tiles;
       }
       units += tiles * P.splits;
     }
     if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
     if (units == 0) continue;
+    if (clear && split_tiles)
+      MX_CU(cudaMemsetAsync(split_count, 0, split_tiles * sizeof(uint32_t), stream));
     g.units = (int32_t)units;
-    if (shape.cg == 2) MX_OK((launch_product<2, EPI>(g, stream)));
-    else MX_OK((launch_product<1, EPI>(g, stream)));
+    MX_OK((launch_product<EPI, DT>(g, pairs, stream)));
   }
   return TA_OK;
 }
@@ -397,8 +428,8 @@ OrthoSpace carve_ortho(OrthoPlan* plan, Arena* a) {
   s.table = a->take<Item>(plan->items);
   s.scale = a->take<Scale>(plan->items);
   s.partial = a->take<double>(plan->chunks);
-  s.split_count = a->take<uint32_t>(kSplitUnits);
-  s.split_ws = a->take<float>(kSplitUnits * kSplitTileBytes / 4);
+  s.split_count = a->take<uint32_t>(kSplitTiles);
+  s.split_ws = a->take<float>(kSplitFloats);
   for (Class& c : plan->classes) {
     c.x0 = a->take<__half>(c.xs() * c.count * (c.pair ? 2 : 1));
     c.x1 = a->take<__half>(c.xs() * c.count);
@@ -457,7 +488,7 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     ta.scale = sp.scale;
     ta.partial = sp.partial;
     ta.zero = sp.split_count;
-    ta.zero_words = lo == 0 ? (int32_t)kSplitUnits : 0;
+    ta.zero_words = lo == 0 ? (int32_t)kSplitTiles : 0;
     int64_t most = 1;
     for (int i = 0; i < ta.count; ++i) most = std::max<int64_t>(most, ta.s[i].batch);
     k_table<<<(unsigned)std::min<int64_t>(cdiv(most, kEltThreads), 64), kEltThreads, 0, stream>>>(ta);
@@ -583,14 +614,14 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     } else {
       sc.alpha = kScaleA / (kScaleX * kScaleX);
     }
-    MX_OK(run_products<EPI_GRAM>(gram(step == 0), false, sc, sp.split_ws, sp.split_count, status,
+    MX_OK(run_products<EPI_GRAM>(gram(step == 0), false, sc, sp.split_ws, sp.split_count, false, status,
                                  stream));
     // a I + b A + c A^2
     sc = Scalars();
     sc.c0 = (float)(kScaleP * abc[0]);
     sc.c1 = (float)(kScaleP * abc[1] / kScaleA);
     sc.c2 = (float)(kScaleP * abc[2] / ((double)kScaleA * kScaleA));
-    MX_OK(run_products<EPI_POLY>(squares(0), false, sc, sp.split_ws, sp.split_count, status,
+    MX_OK(run_products<EPI_POLY>(squares(0), false, sc, sp.split_ws, sp.split_count, false, status,
                                  stream));
     refresh();
     // The first two polynomials act on the unrounded input together: the first iterate, rounded,
@@ -600,7 +631,7 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     if (step == 1) {
       sc = Scalars();
       sc.alpha = 1.f / kScaleP;
-      MX_OK(run_products<EPI_GRAM>(squares(1), false, sc, sp.split_ws, sp.split_count, status,
+      MX_OK(run_products<EPI_GRAM>(squares(1), false, sc, sp.split_ws, sp.split_count, false, status,
                                    stream));
       poly = grams;
     }
@@ -610,7 +641,7 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     if (last) {
       sc.alpha = from_x0 ? 1.f / kScaleP : 1.f / (kScaleP * kScaleX);
       MX_OK(run_products<EPI_FINAL>(apply(poly, x, from_x0, true, x1), false, sc, sp.split_ws,
-                                    sp.split_count, status, stream));
+                                    sp.split_count, false, status, stream));
     } else {
       sc.alpha = from_x0 ? kScaleX / kScaleP : 1.f / kScaleP;
       // the iterate moves to x1; from the third step on its old storage takes the next one
@@ -618,7 +649,7 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
         for (Class& c : plan.classes) std::swap(c.x0, c.x1);
       refresh();
       MX_OK(run_products<EPI_APPLY>(apply(poly, x, from_x0, step == 1, x1), false, sc,
-                                    sp.split_ws, sp.split_count, status, stream));
+                                    sp.split_ws, sp.split_count, false, status, stream));
       if (step == 0)
         for (Class& c : plan.classes) std::swap(c.poly, c.prod);
     }
@@ -711,8 +742,8 @@ ta_status prepare_linear(const ta_linear* op, Lines* x, Lines* w) {
 
 LinearSpace carve_linear(const Lines& x, const Lines& w, Arena* a) {
   LinearSpace s;
-  s.split_count = a->take<uint32_t>(kSplitUnits);
-  s.split_ws = a->take<float>(kSplitUnits * kSplitTileBytes / 4);
+  s.split_count = a->take<uint32_t>(kSplitTiles);
+  s.split_ws = a->take<float>(kSplitFloats);
   s.xc = a->take<uint16_t>(copy_elems(x));
   s.wc = a->take<uint16_t>(copy_elems(w));
   return s;
@@ -728,15 +759,15 @@ ta_status check_space(const Arena& need, void* ws, size_t bytes, const uint32_t*
   return TA_OK;
 }
 
-// The products of one linear call: counters are cleared where a launch may split its sums.
 ta_status plain_product(const Product& p, bool bf16, const LinearSpace& s, uint32_t* status,
                         cudaStream_t stream, bool linear) {
   const std::vector<Product> ps(1, p);
-  if (choose(ps).splits[0] > 1)
-    MX_CU(cudaMemsetAsync(s.split_count, 0, kSplitUnits * sizeof(uint32_t), stream));
+  auto run = [&](auto fn) {
+    return fn(ps, bf16, Scalars(), s.split_ws, s.split_count, true, status, stream);
+  };
   if (linear)
-    return run_products<EPI_LINEAR>(ps, bf16, Scalars(), s.split_ws, s.split_count, status, stream);
-  return run_products<EPI_PLAIN>(ps, bf16, Scalars(), s.split_ws, s.split_count, status, stream);
+    return bf16 ? run(run_products<EPI_LINEAR, DT_BF16>) : run(run_products<EPI_LINEAR, DT_F16>);
+  return bf16 ? run(run_products<EPI_PLAIN, DT_BF16>) : run(run_products<EPI_PLAIN, DT_F16>);
 }
 
 struct GradLines {
@@ -878,7 +909,6 @@ ta_status ta_linear_forward(const ta_linear* op, void* workspace_dev, size_t wor
     p.M = op->tokens;
     p.N = op->fan_out;
     p.ep.za = p.ep.zb = 1;
-    p.ep.dt = (int16_t)op->dtype;
     p.ep.out = op->y_dev;
     p.ep.ldo = (int32_t)op->y_stride;
     p.ep.aux = op->residual_dev;
@@ -957,8 +987,7 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
       p.M = T;
       p.N = I;
       p.ep.za = p.ep.zb = 1;
-      p.ep.dt = (int16_t)op->dtype;
-      p.ep.out = op->dx_dev;
+        p.ep.out = op->dx_dev;
       p.ep.ldo = (int32_t)I;
       MX_OK(plain_product(p, bf16, s.lin, status_dev, stream, false));
     }
@@ -977,8 +1006,7 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
       if (p.M > 1 && ldo > kMaxDim)
         return ta_fail(TA_ERR_UNSUPPORTED, "a row stride is over 2^31 - 256");
       p.ep.za = p.ep.zb = 1;
-      p.ep.dt = (int16_t)op->dtype;
-      p.ep.out = op->dw_dev;
+        p.ep.out = op->dw_dev;
       p.ep.ldo = (int32_t)(p.M > 1 ? ldo : p.N);
       MX_OK(plain_product(p, bf16, s.lin, status_dev, stream, false));
     }
