@@ -95,18 +95,46 @@ struct Operand {
   bool mn_major = false;
 };
 
-// box_mn: rows (or columns) of the output one copy brings; an mn-major operand comes in chunks of 64.
-ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn) {
+// The map one stage of an operand is loaded with: box_mn rows (or columns) of the output by 64
+// k's. *kind: 0 K-major; 1 MN-major, one copy for each chunk of 64; 2 MN-major in one copy, over
+// chunks as a dimension of their own, where the lines are whole chunks (a chunk that ran over the
+// end of a line would read the next one, and past the end of the last).
+ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn, int16_t* kind) {
   EncodeFn fn = encode_fn();
   if (!fn) return ta_fail(TA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-  const int64_t inner = o.mn_major ? o.mn : o.k, lines = o.mn_major ? o.k : o.mn;
-  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)lines, (cuuint64_t)o.z};
-  cuuint64_t strides[2] = {(cuuint64_t)(o.ld * 2),
-                           (cuuint64_t)(std::max<int64_t>(o.zs, o.ld) * 2)};
-  cuuint32_t box[3] = {64, (cuuint32_t)(o.mn_major ? kDepth : box_mn), 1};
-  cuuint32_t step[3] = {1, 1, 1};
-  CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                  const_cast<void*>(o.p), dims, strides, box, step,
+  const cuuint64_t line = (cuuint64_t)o.ld * 2;
+  const cuuint64_t plane = (cuuint64_t)std::max<int64_t>(o.zs, o.ld) * 2;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4] = {64, 64, 1, 1}, step[4] = {1, 1, 1, 1};
+  cuuint32_t rank = 3;
+  if (!o.mn_major) {
+    *kind = 0;
+    dims[0] = (cuuint64_t)o.k;
+    dims[1] = (cuuint64_t)o.mn;
+    box[1] = (cuuint32_t)box_mn;
+  } else if (o.mn % 64) {
+    *kind = 1;
+    dims[0] = (cuuint64_t)o.mn;
+    dims[1] = (cuuint64_t)o.k;
+  } else {
+    *kind = 2;
+    rank = 4;
+    dims[0] = 64;
+    dims[1] = (cuuint64_t)o.k;
+    dims[2] = (cuuint64_t)(o.mn / 64);
+    dims[3] = (cuuint64_t)o.z;
+    strides[0] = line;
+    strides[1] = 128;
+    strides[2] = plane;
+    box[2] = (cuuint32_t)(box_mn / 64);
+  }
+  if (rank == 3) {
+    dims[2] = (cuuint64_t)o.z;
+    strides[0] = line;
+    strides[1] = plane;
+  }
+  CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  rank, const_cast<void*>(o.p), dims, strides, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -144,15 +172,15 @@ struct Shape {
 constexpr int64_t kSplitTiles = 592;                    // counters: one per CTA tile
 constexpr int64_t kSplitFloats = 320ll * kRows * 256;   // partial sums
 
-// SM cycles of a pair's tile of `cols` columns: per block of 64 k's the tensor pipe needs 2 cols
-// and shared memory 256 + cols; each gets in the other's way by about half of the smaller. The
-// epilogue of a single-accumulator tile (cols > 256) is not hidden; a tile costs about 1500 cycles
-// to begin and end.
+// SM cycles of a pair's tile of `cols` columns. A block of 64 k's costs what the slowest of four
+// takes: the tensor pipe (2 cols), shared memory (256 + cols), the copies' issue (about 350) and,
+// where the first two are close, their getting in each other's way (measured 590 cycles at 256
+// columns). The epilogue, some 1500 cycles a chunk for each of four warps, is hidden behind the
+// next tile's products or hides them.
 double tile_cycles(double kblocks, int cols) {
-  const double mma = 2.0 * cols, mem = 256.0 + cols;
-  const double loop = kblocks * (std::max(mma, mem) + 0.5 * std::min(mma, mem) * (mem > 0.9 * mma));
-  const double epilogue = 1000.0 + 12.0 * cols;
-  return cols > 256 ? loop + epilogue + 500 : std::max(loop, epilogue) + 500;
+  const double loop = kblocks * std::max(350.0, std::max(2.0 * cols, 256.0 + cols) + 0.15 * cols);
+  const double epilogue = 1200.0 + 1500.0 * (double)cdiv(cols, 128);
+  return std::max(loop, epilogue) + 0.3 * std::min(loop, epilogue);
 }
 
 // Tile width and splits of a launch: the lowest estimate of (rounds of tiles) x (time of a tile)
@@ -162,9 +190,10 @@ double tile_cycles(double kblocks, int cols) {
 Shape choose(const std::vector<Product>& ps, int pairs) {
   bool b_mn = false;
   for (const Product& p : ps) b_mn = b_mn || p.b.mn_major;
-  static const int kAny[] = {512, 448, 384, 320, 256, 192, 128, 64}, kChunked[] = {512, 256, 128};
+  static const int kAny[] = {256, 224, 192, 160, 128, 96, 64};
+  static const int kChunked[] = {256, 128};  // a CTA's share is whole 64s
   const int* widths = b_mn ? kChunked : kAny;
-  const int n_widths = b_mn ? 3 : 8;
+  const int n_widths = b_mn ? 2 : 7;
   Shape best;
   best.splits.assign(ps.size(), 1);
   double best_time = 1e300;
@@ -218,6 +247,25 @@ Shape choose(const std::vector<Product>& ps, int pairs) {
   return best;
 }
 
+// Launches a kernel of a chain: it may start its set-up while the kernel before it drains (every
+// kernel of this file waits for that one before it touches global memory).
+template <typename... Params, typename... Args>
+ta_status launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                 cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  MX_CU(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
+  return TA_OK;
+}
+
 // Shared-memory limit and resident pairs of an instance, found once per device. A die's SM count
 // need not divide into pairs, so the pairs that fit are asked for: one that had to wait for
 // another to finish would double the time of a persistent launch.
@@ -255,9 +303,7 @@ ta_status pairs_of(int* pairs) {
 template <int EPI, int DT>
 ta_status launch_product(const ProductArgs& g, int pairs, cudaStream_t stream) {
   const unsigned grid = 2u * (unsigned)std::min<int64_t>(g.units, pairs);
-  k_product<EPI, DT><<<grid, kThreads, kProductSmem, stream>>>(g);
-  MX_CU(cudaGetLastError());
-  return TA_OK;
+  return launch(k_product<EPI, DT>, dim3(grid), kThreads, kProductSmem, stream, g);
 }
 
 struct Scalars {
@@ -289,9 +335,6 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
     g.unit_pow = sc.unit_pow;
     g.status = status;
     g.cols = shape.cols;
-    g.halves = shape.cols > 256 ? 2 : 1;
-    g.half = shape.cols / g.halves;
-    g.buffers = shape.cols > 256 ? 1 : 2;
     g.stages = (int)std::min<size_t>(
         kMaxStages, kOperandSpace / (size_t)(kTileABytes + shape.cols * kDepth));
     int64_t units = 0, split_floats = 0, split_tiles = 0;
@@ -300,8 +343,8 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
       Problem& P = g.p[i];
       P = p.ep;
       if (p.a.k > 0) {
-        MX_OK(make_map(&P.ta, p.a, bf16, kRows));
-        MX_OK(make_map(&P.tb, p.b, bf16, g.half / 2));
+        MX_OK(make_map(&P.ta, p.a, bf16, kRows, &P.a_mn));
+        MX_OK(make_map(&P.tb, p.b, bf16, g.cols / 2, &P.b_mn));
       }
       P.M = (int32_t)p.M;
       P.N = (int32_t)p.N;
@@ -313,8 +356,6 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
       P.first = (int32_t)units;
       P.batch = (int32_t)p.batch;
       P.splits = shape.splits[i];
-      P.a_mn = p.a.mn_major;
-      P.b_mn = p.b.mn_major;
       P.sym = p.sym;
       const int64_t tiles = (int64_t)P.tiles * p.batch;
       if (P.splits > 1) {
@@ -491,15 +532,15 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     ta.zero_words = lo == 0 ? (int32_t)kSplitTiles : 0;
     int64_t most = 1;
     for (int i = 0; i < ta.count; ++i) most = std::max<int64_t>(most, ta.s[i].batch);
-    k_table<<<(unsigned)std::min<int64_t>(cdiv(most, kEltThreads), 64), kEltThreads, 0, stream>>>(ta);
-    MX_CU(cudaGetLastError());
+    MX_OK(launch(k_table, dim3((unsigned)std::min<int64_t>(cdiv(most, kEltThreads), 64)),
+                 kEltThreads, 0, stream, ta));
   }
   const float mu = (float)o->momentum;
-  k_norm<<<(unsigned)chunk, kEltThreads, 0, stream>>>(sp.table, (int)plan.items, mu, o->nesterov);
-  MX_CU(cudaGetLastError());
-  k_scale<<<(unsigned)chunk, kEltThreads, 0, stream>>>(sp.table, (int)plan.items, mu, o->nesterov,
-                                                      o->eps);
-  MX_CU(cudaGetLastError());
+  const int items = (int)plan.items;
+  MX_OK(launch(k_norm, dim3((unsigned)chunk), kEltThreads, 0, stream, sp.table, items, mu,
+               o->nesterov));
+  MX_OK(launch(k_scale, dim3((unsigned)chunk), kEltThreads, 0, stream, sp.table, items, mu,
+               o->nesterov, o->eps));
 
   const size_t nc = plan.classes.size();
   auto square = [](const Class& c, const __half* p) {
@@ -699,9 +740,8 @@ ta_status operand_of(const void* p, int64_t mn, int64_t k, const Lines& l, uint1
     o->ld = up8(l.len);
     const dim3 grid((unsigned)std::min<int64_t>(cdiv(l.len, kEltThreads), 64),
                     (unsigned)std::min<int64_t>(l.lines, 4096));
-    k_copy_rows<<<grid, kEltThreads, 0, stream>>>(reinterpret_cast<const uint16_t*>(p), l.stride,
-                                                  (int)l.lines, (int)l.len, copy, (int)o->ld);
-    MX_CU(cudaGetLastError());
+    MX_OK(launch(k_copy_rows, grid, kEltThreads, 0, stream, reinterpret_cast<const uint16_t*>(p),
+                 l.stride, (int)l.lines, (int)l.len, copy, (int)o->ld));
   }
   o->zs = o->ld * l.lines;
   return TA_OK;
@@ -957,16 +997,12 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
     const void* dz = g.make_dz ? (const void*)s.dz : op->dy_dev;
     if (O > 0 && (g.make_dz || op->db_dev)) {
       const dim3 grid((unsigned)cdiv(O, 256), (unsigned)g.row_parts);
-      k_dz<<<grid, kEltThreads, 0, stream>>>(op->dy_dev, op->dy_stride, op->deriv_dev,
-                                             (int)up8(O), (int)T, (int)O, op->dtype,
-                                             g.make_dz ? s.dz : nullptr, (int)g.ld_dz,
-                                             op->db_dev ? s.part : nullptr);
-      MX_CU(cudaGetLastError());
-      if (op->db_dev) {
-        k_bias_grad<<<(unsigned)cdiv(O, kEltThreads), kEltThreads, 0, stream>>>(
-            s.part, (int)g.row_parts, (int)O, op->db_dev, op->bias_dtype);
-        MX_CU(cudaGetLastError());
-      }
+      MX_OK(launch(k_dz, grid, kEltThreads, 0, stream, op->dy_dev, op->dy_stride, op->deriv_dev,
+                   (int)up8(O), (int)T, (int)O, (int)op->dtype, g.make_dz ? s.dz : nullptr,
+                   (int)g.ld_dz, op->db_dev ? s.part : nullptr));
+      if (op->db_dev)
+        MX_OK(launch(k_bias_grad, dim3((unsigned)cdiv(O, kEltThreads)), kEltThreads, 0, stream,
+                     s.part, (int)g.row_parts, (int)O, op->db_dev, (int)op->bias_dtype));
     }
     auto dz_operand = [&](bool over_tokens) {  // summed over tokens (dw) or fan_out (dx)
       Operand o;

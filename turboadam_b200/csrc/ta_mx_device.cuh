@@ -69,6 +69,16 @@ __device__ __forceinline__ void sts_elem(uint32_t a, uint32_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((uint16_t)v) : "memory");
 }
 
+// ---- dependent launches ----
+// A kernel of a chain starts while its predecessor drains: it sets itself up, then waits here
+// before it touches memory that the predecessor reads or writes.
+__device__ __forceinline__ void chain_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void chain_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---- clusters --------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -100,10 +110,11 @@ __device__ __forceinline__ void bar_expect_tx(uint64_t* b, uint32_t bytes) {
                "r"(bytes)
                : "memory");
 }
-// Arrive on a barrier of any CTA of the cluster (shared::cluster address).
+// Arrive on a barrier of any CTA of the cluster (shared::cluster address). What it orders is the
+// thread's tensor-memory reads (behind tc_fence_before), not its global stores: a release at
+// cluster scope would wait about 1000 cycles for those.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
-               : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t bar_try(uint64_t* b, uint32_t parity) {
   uint32_t ok;
@@ -134,47 +145,35 @@ __device__ __forceinline__ void tma_prefetch(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
 // One box of a 3-D tensor map into this CTA's shared memory; its bytes are counted on the
-// barrier at shared::cluster address `bar` (with CG == 2: of either CTA of the pair).
-template <int CG>
+// barrier at shared::cluster address `bar`, of either CTA of the pair.
 __device__ __forceinline__ void tma_load(const CUtensorMap* m, uint32_t dst, uint32_t bar, int x,
                                          int y, int z) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
-        "bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z)
-        : "memory");
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// The same of a 4-D map whose innermost dimension is taken whole.
+__device__ __forceinline__ void tma_load4(const CUtensorMap* m, uint32_t dst, uint32_t bar, int y,
+                                          int z, int t) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(0), "r"(y), "r"(z), "r"(t)
+      : "memory");
 }
 
-// ---- tcgen05 ---------------------------------------------------------------
-template <int CG>
+// ---- tcgen05 (pairs of SMs) ----------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
-  if constexpr (CG == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(slot)),
-                 "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  } else {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(slot)),
-                 "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-  }
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_addr(slot)),
+               "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
 }
-template <int CG>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
-  if constexpr (CG == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
-  else
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -182,56 +181,23 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// D[tmem] (+)= A[smem] B[smem], 16-bit operands, fp32 accumulators, K = 16.
-template <int CG>
+// D[tmem] (+)= A[smem] B[smem] on a pair of SMs, 16-bit operands, fp32 accumulators, K = 16.
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        bool accumulate) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-// The same on a pair of SMs, leaving A in the collector for the next instruction, and taking it
-// from there (same descriptor of A).
-__device__ __forceinline__ void tc_mma_fill(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                            bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16.collector::a::fill [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_last(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                            bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16.collector::a::lastuse [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-// Arrive on `bar` (with CG == 2: on the barrier at that offset in both CTAs of the pair) when
-// every matrix instruction issued so far by this thread has finished.
-template <int CG>
+// Arrive on the barrier at `bar`'s offset in both CTAs of the pair when every matrix instruction
+// issued so far by this thread has finished.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-            smem_addr(bar))
-        : "memory");
-  else
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;" ::"r"(smem_addr(bar)),
-        "h"((uint16_t)3)
-        : "memory");
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
 }
 // 32 consecutive columns of this warp's 32 tensor-memory lanes: lane l gets row l.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {

@@ -36,6 +36,8 @@ __device__ __forceinline__ const void* offset_dt(const void* p, int64_t elems, i
 }
 
 __global__ void __launch_bounds__(kEltThreads) k_table(const __grid_constant__ TableArgs a) {
+  chain_next();
+  chain_wait();
   const int t = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
   for (int i = t; i < a.zero_words; i += stride) a.zero[i] = 0;
   for (int k = 0; k < a.count; ++k) {
@@ -129,6 +131,8 @@ __device__ __forceinline__ bool item_vec(const Item& it) {
 // fp32's range keep their norm.
 __global__ void __launch_bounds__(kEltThreads)
     k_norm(const Item* table, int count, float mu, int nesterov) {
+  chain_next();
+  chain_wait();
   const Item& it = find_item(table, count, blockIdx.x);
   const int chunk = blockIdx.x - it.chunk0;
   const int64_t e0 = chunk * it.chunk_elems, e1 = min(it.n, e0 + it.chunk_elems);
@@ -171,6 +175,8 @@ __global__ void __launch_bounds__(kEltThreads)
 // numbers where x0_lo is given (22 bits) and rounded once otherwise.
 __global__ void __launch_bounds__(kEltThreads)
     k_scale(const Item* table, int count, float mu, int nesterov, double eps) {
+  chain_next();
+  chain_wait();
   const Item& it = find_item(table, count, blockIdx.x);
   const int chunk = blockIdx.x - it.chunk0;
   const double norm = sqrt(block_sum((int)threadIdx.x < it.chunks ? it.partial[threadIdx.x] : 0.0));
@@ -219,6 +225,8 @@ __global__ void __launch_bounds__(kEltThreads)
 // rows x cols 16-bit elements into rows of ld elements (TMA reads rows that start on 16 bytes).
 __global__ void __launch_bounds__(kEltThreads)
     k_copy_rows(const uint16_t* src, int64_t stride, int rows, int cols, uint16_t* dst, int ld) {
+  chain_next();
+  chain_wait();
   for (int r = blockIdx.y; r < rows; r += gridDim.y)
     for (int c = blockIdx.x * kEltThreads + threadIdx.x; c < cols; c += gridDim.x * kEltThreads)
       dst[(int64_t)r * ld + c] = src[(int64_t)r * stride + c];
@@ -231,6 +239,8 @@ __global__ void __launch_bounds__(kEltThreads)
 __global__ void __launch_bounds__(kEltThreads)
     k_dz(const void* dy, int64_t dy_stride, const int16_t* deriv, int ld_deriv, int rows, int cols,
          int dt, uint16_t* dz, int ld_dz, float* part) {
+  chain_next();
+  chain_wait();
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
   const int c0 = blockIdx.x * 256 + lane * 8;
   const int r0 = (int)((int64_t)rows * blockIdx.y / gridDim.y);
@@ -277,6 +287,8 @@ __global__ void __launch_bounds__(kEltThreads)
 }
 __global__ void __launch_bounds__(kEltThreads)
     k_bias_grad(const float* part, int parts, int cols, void* db, int dt) {
+  chain_next();
+  chain_wait();
   const int c = blockIdx.x * kEltThreads + threadIdx.x;
   if (c >= cols) return;
   float t = 0;
