@@ -50,9 +50,9 @@ enum {
  *   A <- X X^T (X^T X if rows > cols);  X <- (a I + b A + c A^2) X
  *   O <- X
  * The products run on fp16 operands (X, A and the polynomial, each scaled by
- * a power of two) with fp32 sums; X enters unrounded (16-bit inputs) and the
- * first two polynomials act on it as one, so the first iterate is not rounded
- * either. Their relative error is about 1e-3 of O; bf16 operands would leave
+ * a power of two) with fp32 sums; X enters unrounded (16-bit inputs), and the
+ * steps act in pairs, X <- P' P X with the second Gram matrix formed from the
+ * first. The relative error is about 1.5e-3 of O; bf16 operands would leave
  * 1e-2 to 3e-2. A zero matrix gives zero; a NaN or an infinity in a matrix
  * makes all of that matrix's O NaN.
  */
@@ -78,8 +78,8 @@ typedef struct ta_ortho_options {
 TA_API size_t ta_ortho_workspace_size(const ta_ortho_tensor* tensors, int32_t n_tensors,
                                       const ta_ortho_options* options);
 
-/* Orthogonalises (and, with TA_ORTHO_UPDATE, applies) the whole list in 3 * steps + 4 launches
- * per 8 distinct shapes. */
+/* Orthogonalises (and, with TA_ORTHO_UPDATE, applies) the whole list: for every 8 distinct shapes
+ * 7 launches for two steps, 3 for a last odd one, and 3 or more launches before them. */
 TA_API ta_status ta_orthogonalize(const ta_ortho_tensor* tensors, int32_t n_tensors,
                                   const ta_ortho_options* options, void* workspace_dev,
                                   size_t workspace_bytes, uint32_t* status_dev, void* stream);

@@ -17,6 +17,7 @@
 #include "../../include/turboadam_b200_matrix.h"
 #include "ta_host.h"
 #include "ta_mx_elementwise.cuh"
+#include "ta_mx_few.cuh"
 #include "ta_mx_product.cuh"
 
 using namespace ta::mx;
@@ -37,6 +38,7 @@ namespace {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t up8(int64_t x) { return (x + 7) & ~(int64_t)7; }
+inline int64_t up32(int64_t x) { return (x + 31) & ~(int64_t)31; }
 inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline int64_t dt_bytes(int dt) { return dt == TA_F32 ? 4 : 2; }
@@ -149,7 +151,8 @@ struct Product {
   int parts = 1;
   bool sym = false;
   int64_t batch = 1;
-  Problem ep;  // the epilogue's fields
+  bool padded = false;  // the result's lines have room for whole chunks
+  Problem ep;           // the epilogue's fields
   Product() { memset(&ep, 0, sizeof(ep)); }
 };
 
@@ -348,6 +351,7 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
       }
       P.M = (int32_t)p.M;
       P.N = (int32_t)p.N;
+      P.n_end = (int32_t)(p.padded ? up32(p.N) : p.N);
       P.kblocks = (int32_t)cdiv(p.a.k, kDepth);
       P.parts = p.parts;
       P.tiles_m = (int32_t)cdiv(p.M, kTileRows);
@@ -380,7 +384,8 @@ ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars
 // Scales of the fp16 matrices: X, the Gram matrix and the polynomial are at most a few units in
 // norm (the quintic keeps singular values below 1.3), so 2^10 and 2^8 leave 2^6 to 2^8 of head
 // room under fp16's largest number and put elements of 2^-24 and 2^-22 on its smallest normal.
-constexpr float kScaleX = 1024.f, kScaleA = 1024.f, kScaleP = 256.f;
+// (The product of two polynomials is at most the square of one, P A a few times A.)
+constexpr float kScaleX = 1024.f, kScaleA = 1024.f, kScaleP = 256.f, kScaleT = 512.f;
 
 struct Class {  // matrices of one shape
   int64_t rows = 0, cols = 0, ld = 0, side = 0, lds = 0, count = 0;
@@ -399,7 +404,7 @@ struct OrthoPlan {
 };
 
 int64_t chunk_elems(int64_t n) {
-  return std::max<int64_t>(8192, cdiv(cdiv(n, kMaxChunks), 2048) * 2048);
+  return std::max<int64_t>(4096, cdiv(cdiv(n, kMaxChunks), 2048) * 2048);
 }
 
 ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_options* o,
@@ -435,10 +440,10 @@ ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_option
       Class c;
       c.rows = t.rows;
       c.cols = t.cols;
-      c.ld = up8(t.cols);
+      c.ld = up32(t.cols);  // whole epilogue chunks
       c.tall = t.rows > t.cols;
       c.side = std::min(t.rows, t.cols);
-      c.lds = up8(c.side);
+      c.lds = up32(c.side);
       c.pair = pair;
       plan->classes.push_back(c);
       plan->members.emplace_back();
@@ -564,15 +569,17 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     q.mn_major = sum_over_rows;
     return q;
   };
-  // out = left * right of side x side matrices (or the Gram matrix of the iterate), symmetric
-  auto gram = [&](bool first) {  // A from X; the first iterate is x0 (its upper half, if a pair)
+  // A from X; the first iterate is x0 (its upper half, if a pair)
+  auto gram = [&](bool first) {
     std::vector<Product> ps;
     for (const Class& c : plan.classes) {
       Product p;
       const bool pair = c.pair && first;
       p.a = iterate(c, first ? c.x0 : c.x1, c.tall, c.count * (pair ? 2 : 1));
       p.b = p.a;
-      p.M = p.N = c.side;
+      p.M = c.side;
+      p.N = c.side;
+      p.padded = true;
       p.sym = true;
       p.batch = c.count;
       p.ep.za = p.ep.zb = pair ? 2 : 1;
@@ -584,20 +591,24 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     }
     return ps;
   };
-  auto squares = [&](int which) {  // 0: the polynomial from A; 1: its product with the last one
+  // out = a b of side x side matrices that commute, so that it is symmetric too
+  using Square = __half* Class::*;
+  auto squares = [&](Square a, Square b, Square out) {
     std::vector<Product> ps;
     for (const Class& c : plan.classes) {
       Product p;
-      p.a = square(c, which == 0 ? c.gram : c.poly);
-      p.b = square(c, which == 0 ? c.gram : c.prod);
-      p.M = p.N = c.side;
+      p.a = square(c, c.*a);
+      p.b = square(c, c.*b);
+      p.M = c.side;
+      p.N = c.side;
+      p.padded = true;
       p.sym = true;
       p.batch = c.count;
       p.ep.za = p.ep.zb = 1;
-      p.ep.out = which == 0 ? c.poly : c.gram;
+      p.ep.out = c.*out;
       p.ep.out_zs = c.ss();
       p.ep.ldo = (int32_t)c.lds;
-      p.ep.aux = c.gram;
+      p.ep.aux = c.*a;
       p.ep.aux_zs = c.ss();
       p.ep.ld_aux = (int32_t)c.lds;
       p.ep.scale = sp.scale + c.first;
@@ -607,24 +618,22 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
   };
   // X <- poly * x (x * poly, if tall); from_x0: x is the scaled input, with both parts of a pair
   // if `whole`
-  auto apply = [&](const std::vector<__half*>& poly, const std::vector<__half*>& x, bool from_x0,
-                   bool whole, const std::vector<__half*>& out) {
+  auto apply = [&](Square poly, bool first) {
     std::vector<Product> ps;
-    for (size_t i = 0; i < nc; ++i) {
-      const Class& c = plan.classes[i];
+    for (const Class& c : plan.classes) {
       Product p;
-      const bool pair = c.pair && from_x0;
-      const Operand q = square(c, poly[i]);
-      const Operand v = iterate(c, x[i], !c.tall, c.count * (pair ? 2 : 1));
+      const bool pair = c.pair && first;
+      const Operand q = square(c, c.*poly);
+      const Operand v = iterate(c, first ? c.x0 : c.x1, !c.tall, c.count * (pair ? 2 : 1));
       p.a = c.tall ? v : q;
       p.b = c.tall ? q : v;
-      p.parts = pair && whole ? 2 : 1;
+      p.parts = pair ? 2 : 1;
       p.M = c.rows;
       p.N = c.cols;
       p.batch = c.count;
       p.ep.za = c.tall && pair ? 2 : 1;
       p.ep.zb = !c.tall && pair ? 2 : 1;
-      p.ep.out = out[i];
+      p.ep.out = first ? c.x1 : c.x0;
       p.ep.out_zs = c.xs();
       p.ep.ldo = (int32_t)c.ld;
       p.ep.scale = sp.scale + c.first;
@@ -634,65 +643,55 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     return ps;
   };
 
-  std::vector<__half*> x0(nc), x1(nc), polys(nc), prods(nc), grams(nc);
-  auto refresh = [&] {
-    for (size_t i = 0; i < nc; ++i) {
-      x0[i] = plan.classes[i].x0;
-      x1[i] = plan.classes[i].x1;
-      polys[i] = plan.classes[i].poly;
-      prods[i] = plan.classes[i].prod;
-      grams[i] = plan.classes[i].gram;
-    }
-  };
-  for (int step = 0; step < o->steps; ++step) {
-    const double* abc = o->coefficients + 3 * step;
-    const bool last = step == o->steps - 1;
+  // Steps go in pairs. With A the Gram matrix of X, P and P' the polynomials of two steps,
+  //   T = P A,  A' = P T  (the Gram matrix of P X, without forming P X),  Q = P' P,  X <- Q X:
+  // in units of a side^3 product and with r = long / short side, 3 r + 5 for two steps against
+  // 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the unrounded
+  // input. Rounding A, and not X, costs accuracy where A's small eigenvalues drown in the error
+  // of its large ones; over two steps (with the input exact) they do not: 1.3e-3 to 1.7e-3 of the
+  // result on spectra that decay by 50 to 800, against 1.8e-3 to 2.6e-3 one by one (bf16
+  // operands: 2e-2). Over three they would (1e-2).
+  auto run = [&](auto fn, const std::vector<Product>& ps, float alpha, int unit_pow) {
     Scalars sc;
-    // A
-    if (step == 0) {
-      sc.alpha = kScaleA;
-      sc.unit_pow = 2;
-    } else {
-      sc.alpha = kScaleA / (kScaleX * kScaleX);
-    }
-    MX_OK(run_products<EPI_GRAM>(gram(step == 0), false, sc, sp.split_ws, sp.split_count, false, status,
-                                 stream));
-    // a I + b A + c A^2
-    sc = Scalars();
+    sc.alpha = alpha;
+    sc.unit_pow = unit_pow;
+    return fn(ps, false, sc, sp.split_ws, sp.split_count, false, status, stream);
+  };
+  auto polynomial = [&](int step) {
+    const double* abc = o->coefficients + 3 * step;
+    Scalars sc;
     sc.c0 = (float)(kScaleP * abc[0]);
     sc.c1 = (float)(kScaleP * abc[1] / kScaleA);
     sc.c2 = (float)(kScaleP * abc[2] / ((double)kScaleA * kScaleA));
-    MX_OK(run_products<EPI_POLY>(squares(0), false, sc, sp.split_ws, sp.split_count, false, status,
-                                 stream));
-    refresh();
-    // The first two polynomials act on the unrounded input together: the first iterate, rounded,
-    // only serves the second Gram matrix, whose rounding the result hardly feels.
-    std::vector<__half*> poly = polys, x = x1;
-    const bool from_x0 = step <= 1;
-    if (step == 1) {
-      sc = Scalars();
-      sc.alpha = 1.f / kScaleP;
-      MX_OK(run_products<EPI_GRAM>(squares(1), false, sc, sp.split_ws, sp.split_count, false, status,
-                                   stream));
-      poly = grams;
+    return run_products<EPI_POLY>(squares(&Class::gram, &Class::gram, &Class::poly), false, sc,
+                                  sp.split_ws, sp.split_count, false, status, stream);
+  };
+  for (int step = 0; step < o->steps;) {
+    const bool first = step == 0, two = step + 1 < o->steps;
+    MX_OK(run(run_products<EPI_GRAM>, gram(first),
+              first ? kScaleA : kScaleA / (kScaleX * kScaleX), first ? 2 : 0));
+    MX_OK(polynomial(step));
+    if (two) {
+      MX_OK(run(run_products<EPI_GRAM>, squares(&Class::poly, &Class::gram, &Class::prod),
+                kScaleT / (kScaleP * kScaleA), 0));
+      MX_OK(run(run_products<EPI_GRAM>, squares(&Class::poly, &Class::prod, &Class::gram),
+                kScaleA / (kScaleP * kScaleT), 0));
+      for (Class& c : plan.classes) std::swap(c.poly, c.prod);  // P
+      MX_OK(polynomial(step + 1));                              // P'
+      MX_OK(run(run_products<EPI_GRAM>, squares(&Class::poly, &Class::prod, &Class::gram),
+                1.f / kScaleP, 0));
+      for (Class& c : plan.classes) std::swap(c.poly, c.gram);  // Q
     }
-    if (from_x0) x = x0;
-    sc = Scalars();
-    sc.unit_pow = from_x0 ? 1 : 0;
-    if (last) {
-      sc.alpha = from_x0 ? 1.f / kScaleP : 1.f / (kScaleP * kScaleX);
-      MX_OK(run_products<EPI_FINAL>(apply(poly, x, from_x0, true, x1), false, sc, sp.split_ws,
-                                    sp.split_count, false, status, stream));
+    step += two ? 2 : 1;
+    const float alpha = first ? 1.f / kScaleP : 1.f / (kScaleP * kScaleX);
+    if (step == o->steps) {
+      MX_OK(run(run_products<EPI_FINAL>, apply(&Class::poly, first), alpha, first ? 1 : 0));
     } else {
-      sc.alpha = from_x0 ? kScaleX / kScaleP : 1.f / kScaleP;
-      // the iterate moves to x1; from the third step on its old storage takes the next one
-      if (step >= 2)
+      MX_OK(run(run_products<EPI_APPLY>, apply(&Class::poly, first), alpha * kScaleX,
+                first ? 1 : 0));
+      // the iterate is in x1 from now on; x0 takes the next one
+      if (!first)
         for (Class& c : plan.classes) std::swap(c.x0, c.x1);
-      refresh();
-      MX_OK(run_products<EPI_APPLY>(apply(poly, x, from_x0, step == 1, x1), false, sc,
-                                    sp.split_ws, sp.split_count, false, status, stream));
-      if (step == 0)
-        for (Class& c : plan.classes) std::swap(c.poly, c.prod);
     }
   }
   return TA_OK;
@@ -799,8 +798,66 @@ ta_status check_space(const Arena& need, void* ws, size_t bytes, const uint32_t*
   return TA_OK;
 }
 
+// A few rows of A against all of B: up to 8, read where they lie.
+bool few_rows(const Product& p) {
+  if (p.M < 1 || p.M > kFewMax || p.a.k < 1) return false;
+  if (p.a.mn_major && p.M > 1) return false;
+  if (!aligned16(p.a.p) || (p.M > 1 && p.a.ld % 8)) return false;
+  return p.b.mn_major ? p.N % 8 == 0 : p.a.k % 8 == 0;  // (B's lines start on 16 bytes)
+}
+
+template <int DT, int T>
+ta_status launch_few(FewArgs& g, bool cols, int64_t room, cudaStream_t stream) {
+  const int sms = sm_count();
+  if (!cols) {
+    // enough blocks for two on every SM, by letting warps share a sum where N is small
+    g.warps_n = 8;
+    while (g.warps_n > 1 && cdiv(g.N, g.warps_n * kFewRows) < 2 * sms) g.warps_n /= 2;
+    return launch(k_few_rows<DT, T>, dim3((unsigned)cdiv(g.N, g.warps_n * kFewRows)), 256, 0,
+                  stream, g);
+  }
+  const int64_t blocks = cdiv(g.N, 256);
+  int64_t splits = std::min<int64_t>(cdiv(4 * sms, blocks), cdiv(g.K, 32));
+  splits = std::min(splits, room / ((int64_t)g.tokens * g.N));
+  g.splits = (int)std::max<int64_t>(1, splits);
+  MX_OK(launch(k_few_cols<DT, T>, dim3((unsigned)blocks, (unsigned)g.splits), 256, 0, stream, g));
+  return launch(k_few_finish<DT>, dim3((unsigned)blocks, (unsigned)g.tokens), 256, 0, stream, g);
+}
+
+template <int DT>
+ta_status run_few(const Product& p, float* part, int64_t room, cudaStream_t stream) {
+  FewArgs g;
+  memset(&g, 0, sizeof(g));
+  g.a = reinterpret_cast<const uint16_t*>(p.a.p);
+  g.b = reinterpret_cast<const uint16_t*>(p.b.p);
+  g.lda = p.a.ld;
+  g.ldb = p.b.ld;
+  g.tokens = (int)p.M;
+  g.N = (int)p.N;
+  g.K = (int)p.a.k;
+  g.part = part;
+  g.out = reinterpret_cast<uint16_t*>(p.ep.out);
+  g.aux = reinterpret_cast<const uint16_t*>(p.ep.aux);
+  g.bias = p.ep.bias;
+  g.deriv = p.ep.deriv;
+  g.ldo = p.ep.ldo;
+  g.ld_aux = p.ep.ld_aux;
+  g.ld_deriv = p.ep.ld_deriv;
+  g.bias_dt = p.ep.bias_dt;
+  g.act = p.ep.act;
+  const bool cols = p.b.mn_major;
+  if (g.tokens == 1) return launch_few<DT, 1>(g, cols, room, stream);
+  if (g.tokens == 2) return launch_few<DT, 2>(g, cols, room, stream);
+  if (g.tokens <= 4) return launch_few<DT, 4>(g, cols, room, stream);
+  return launch_few<DT, 8>(g, cols, room, stream);
+}
+
+// The products of one linear call: counters are cleared where a launch may split its sums.
 ta_status plain_product(const Product& p, bool bf16, const LinearSpace& s, uint32_t* status,
                         cudaStream_t stream, bool linear) {
+  if (few_rows(p) && p.M * p.N <= kSplitFloats)
+    return bf16 ? run_few<DT_BF16>(p, s.split_ws, kSplitFloats, stream)
+                : run_few<DT_F16>(p, s.split_ws, kSplitFloats, stream);
   const std::vector<Product> ps(1, p);
   auto run = [&](auto fn) {
     return fn(ps, bf16, Scalars(), s.split_ws, s.split_count, true, status, stream);

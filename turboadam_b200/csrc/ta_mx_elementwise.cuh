@@ -9,7 +9,7 @@ namespace ta {
 namespace mx {
 
 constexpr int kEltThreads = 256;
-constexpr int kMaxChunks = 256;  // partial sums of one matrix (one per thread of a block)
+constexpr int kMaxChunks = 1024;  // partial sums of one matrix
 
 // ---- table ---------------------------------------------------------------------
 // The items of a list travel as kernel parameters and are written to the workspace by a
@@ -82,6 +82,8 @@ __device__ __forceinline__ double block_sum(double v) {
   return s;
 }
 
+constexpr int kUnroll = 4;
+
 struct alignas(16) F8 {
   float v[8];
 };
@@ -137,31 +139,54 @@ __global__ void __launch_bounds__(kEltThreads)
   const int chunk = blockIdx.x - it.chunk0;
   const int64_t e0 = chunk * it.chunk_elems, e1 = min(it.n, e0 + it.chunk_elems);
   double sum = 0;
+  const bool mom = it.mom != nullptr;
   if (item_vec(it)) {
-    for (int64_t i = e0 + threadIdx.x * 8; i < e1; i += kEltThreads * 8) {
-      F8 g = load8(it.g, i, it.g_dt);
-      if (it.mom) {
-        F8 m = load8(it.mom, i, it.mom_dt);
+    // four stretches at a time: their loads are under way together
+    for (int64_t i0 = e0 + threadIdx.x * 8; i0 < e1; i0 += kEltThreads * 8 * kUnroll) {
+      F8 g[kUnroll], m[kUnroll];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          m.v[k] = as_stored(fmaf(mu, m.v[k], (1.f - mu) * g.v[k]), it.mom_dt);
-          g.v[k] = direction(g.v[k], m.v[k], mu, nesterov);
-        }
-        store8(it.mom, i, it.mom_dt, m);
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads * 8;
+        if (i >= e1) continue;
+        g[q] = load8(it.g, i, it.g_dt);
+        if (mom) m[q] = load8(it.mom, i, it.mom_dt);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum = fma((double)g.v[k], (double)g.v[k], sum);
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads * 8;
+        if (i >= e1) continue;
+        if (mom) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            m[q].v[k] = as_stored(fmaf(mu, m[q].v[k], (1.f - mu) * g[q].v[k]), it.mom_dt);
+            g[q].v[k] = direction(g[q].v[k], m[q].v[k], mu, nesterov);
+          }
+          store8(it.mom, i, it.mom_dt, m[q]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum = fma((double)g[q].v[k], (double)g[q].v[k], sum);
+      }
     }
   } else {
-    for (int64_t i = e0 + threadIdx.x; i < e1; i += kEltThreads) {
-      float u = load_as_float(it.g, i, it.g_dt);
-      if (it.mom) {
-        const float m = as_stored(fmaf(mu, load_as_float(it.mom, i, it.mom_dt), (1.f - mu) * u),
-                                  it.mom_dt);
-        store_from_float(it.mom, i, it.mom_dt, m);
-        u = direction(u, m, mu, nesterov);
+    for (int64_t i0 = e0 + threadIdx.x; i0 < e1; i0 += kEltThreads * kUnroll) {
+      float u[kUnroll], m[kUnroll];
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads;
+        u[q] = i < e1 ? load_as_float(it.g, i, it.g_dt) : 0.f;
+        m[q] = mom && i < e1 ? load_as_float(it.mom, i, it.mom_dt) : 0.f;
       }
-      sum = fma((double)u, (double)u, sum);
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads;
+        if (i >= e1) continue;
+        if (mom) {
+          m[q] = as_stored(fmaf(mu, m[q], (1.f - mu) * u[q]), it.mom_dt);
+          store_from_float(it.mom, i, it.mom_dt, m[q]);
+          u[q] = direction(u[q], m[q], mu, nesterov);
+        }
+        sum = fma((double)u[q], (double)u[q], sum);
+      }
     }
   }
   sum = block_sum(sum);
@@ -179,7 +204,9 @@ __global__ void __launch_bounds__(kEltThreads)
   chain_wait();
   const Item& it = find_item(table, count, blockIdx.x);
   const int chunk = blockIdx.x - it.chunk0;
-  const double norm = sqrt(block_sum((int)threadIdx.x < it.chunks ? it.partial[threadIdx.x] : 0.0));
+  double mine = 0;
+  for (int i = threadIdx.x; i < it.chunks; i += kEltThreads) mine += it.partial[i];
+  const double norm = sqrt(block_sum(mine));
   float pow2 = 1.f, unit = 0.f;
   if (!(norm <= 1.7e308)) {
     unit = __int_as_float(0x7fc00000);
@@ -189,34 +216,62 @@ __global__ void __launch_bounds__(kEltThreads)
   }
   if (chunk == 0 && threadIdx.x == 0) *it.scale = Scale{pow2, unit};
   const int64_t e0 = chunk * it.chunk_elems, e1 = min(it.n, e0 + it.chunk_elems);
-  if (item_vec(it) && it.cols == it.ld) {
-    for (int64_t i = e0 + threadIdx.x * 8; i < e1; i += kEltThreads * 8) {
-      F8 g = load8(it.g, i, it.g_dt);
-      if (it.mom) {
-        const F8 m = load8(it.mom, i, it.mom_dt);
+  const bool mom = it.mom != nullptr;
+  // element i's place in the scaled matrix, whose lines are padded to ld
+  auto place = [&](int64_t i) {
+    if (it.cols == it.ld) return i;
+    const int64_t r = it.n <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)it.cols)
+                                         : i / it.cols;
+    return r * it.ld + (i - r * it.cols);
+  };
+  if (item_vec(it) && it.cols % 8 == 0) {
+    for (int64_t i0 = e0 + threadIdx.x * 8; i0 < e1; i0 += kEltThreads * 8 * kUnroll) {
+      F8 g[kUnroll], m[kUnroll];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g.v[k] = direction(g.v[k], m.v[k], mu, nesterov);
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads * 8;
+        if (i >= e1) continue;
+        g[q] = load8(it.g, i, it.g_dt);
+        if (mom) m[q] = load8(it.mom, i, it.mom_dt);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) g.v[k] *= pow2;
-      store8(it.x0, i, DT_F16, g);
-      if (it.x0_lo) {
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads * 8;
+        if (i >= e1) continue;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g.v[k] -= __half2float(__float2half_rn(g.v[k]));
-        store8(it.x0_lo, i, DT_F16, g);
+        for (int k = 0; k < 8; ++k) {
+          if (mom) g[q].v[k] = direction(g[q].v[k], m[q].v[k], mu, nesterov);
+          g[q].v[k] *= pow2;
+        }
+        const int64_t at = place(i);
+        store8(it.x0, at, DT_F16, g[q]);
+        if (it.x0_lo) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) g[q].v[k] -= __half2float(__float2half_rn(g[q].v[k]));
+          store8(it.x0_lo, at, DT_F16, g[q]);
+        }
       }
     }
   } else {
-    for (int64_t i = e0 + threadIdx.x; i < e1; i += kEltThreads) {
-      float u = load_as_float(it.g, i, it.g_dt);
-      if (it.mom) u = direction(u, load_as_float(it.mom, i, it.mom_dt), mu, nesterov);
-      u *= pow2;
-      const int64_t r = it.n <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)it.cols)
-                                           : i / it.cols;
-      const int64_t at = r * it.ld + (i - r * it.cols);
-      const __half hi = __float2half_rn(u);
-      it.x0[at] = hi;
-      if (it.x0_lo) it.x0_lo[at] = __float2half_rn(u - __half2float(hi));
+    for (int64_t i0 = e0 + threadIdx.x; i0 < e1; i0 += kEltThreads * kUnroll) {
+      float u[kUnroll], m[kUnroll];
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads;
+        u[q] = i < e1 ? load_as_float(it.g, i, it.g_dt) : 0.f;
+        m[q] = mom && i < e1 ? load_as_float(it.mom, i, it.mom_dt) : 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int64_t i = i0 + q * kEltThreads;
+        if (i >= e1) continue;
+        if (mom) u[q] = direction(u[q], m[q], mu, nesterov);
+        u[q] *= pow2;
+        const int64_t at = place(i);
+        const __half hi = __float2half_rn(u[q]);
+        it.x0[at] = hi;
+        if (it.x0_lo) it.x0_lo[at] = __float2half_rn(u[q] - __half2float(hi));
+      }
     }
   }
 }

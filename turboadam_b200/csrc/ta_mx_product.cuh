@@ -88,6 +88,7 @@ struct Item {
 struct alignas(64) Problem {
   CUtensorMap ta, tb;
   int32_t M, N;
+  int32_t n_end;            // columns the epilogue writes: N, or whole chunks of padded lines
   int32_t kblocks;          // blocks of 64 k's in one part of the sum
   int32_t parts;            // the sum runs over this many operand pairs
   int32_t tiles_m, tiles_n, tiles;  // per matrix (tiles: on and above the diagonal, if sym)
@@ -479,7 +480,7 @@ __device__ __forceinline__ void finish_linear(const Out& o, const Block& b, floa
 template <int EPI, int DT>
 __device__ __forceinline__ void finish(const ProductArgs& g, const Out& o, const Item* it,
                                        const Block& b, float (&v)[32], float alpha, int64_t row0,
-                                       int col, int n, bool mirror, int64_t N) {
+                                       int col, int n, bool mirror, int N) {
   if constexpr (EPI == EPI_GRAM || EPI == EPI_POLY || EPI == EPI_APPLY) {
     if constexpr (EPI == EPI_POLY) {
       block_load<2>(b, o.aux + (row0 * o.ld_aux + col) * 2, o.ld_aux, n);
@@ -496,7 +497,7 @@ __device__ __forceinline__ void finish(const ProductArgs& g, const Out& o, const
       __half* t = reinterpret_cast<__half*>(o.out) + col * o.ld + row0 + b.lane;
 #pragma unroll
       for (int i = 0; i < 32; ++i, t += o.ld)
-        if (i < n) *t = __float2half_rn(v[i]);
+        if (i < N - col) *t = __float2half_rn(v[i]);  // n may run into the lines' padding
     }
     block_store<2>(b, o.out + (row0 * o.ld + col) * 2, o.ld, n);
   } else if constexpr (EPI == EPI_FINAL) {
@@ -672,7 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int buf = tile & 1;
       const uint32_t use = tile >> 1;
       const int64_t row0 = w.m0 + (int)rank * kRows + quad * 32;
-      const int N = P.N, splits = P.splits;
+      const int N = P.N, n_end = P.n_end, splits = P.splits;
       const bool sym = P.sym;
       b.rows = (int)max((int64_t)0, min((int64_t)32, P.M - row0));
       Out o;
@@ -702,7 +703,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // the result and not left of a symmetric result's diagonal block
       auto wanted = [&](int c) {
         const int col = w.n0 + c;
-        return col < N && b.rows > 0 && !(sym && col < w.m0);
+        return col < n_end && b.rows > 0 && !(sym && col < w.m0);
       };
       a.last = -1;
       if (splits == 1)
@@ -751,7 +752,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int col = w.n0 + c;
           float v[32];
           take_sums(a, c, v);
-          finish<EPI, DT>(g, o, item, b, v, alpha, row0, col, min(32, N - col),
+          finish<EPI, DT>(g, o, item, b, v, alpha, row0, col, min(32, n_end - col),
                           sym && col >= w.m0 + kTileRows, N);
         }
       }

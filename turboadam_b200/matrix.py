@@ -11,6 +11,8 @@ fallback. None has a counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import math
+import struct
 
 import torch
 
@@ -28,16 +30,20 @@ _ACTIVATIONS = {None: _lib.TA_ACT_NONE, "none": _lib.TA_ACT_NONE, "relu": _lib.T
                 "silu": _lib.TA_ACT_SILU}
 
 _status = {}  # device index -> int32 [1], OR-ed into by every call on that device
+_words = {}   # device index -> its address
 
 
-def status_word(device: torch.device) -> torch.Tensor:
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    st = _status.get(idx)
-    if st is None:
-        st = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        torch.cuda.synchronize(st.device)  # zeroed before any stream uses it
-        _status[idx] = st
-    return st
+def _word(index: int) -> int:
+    """Address of the device's status word, zeroed before any stream uses it."""
+    at = _words.get(index)
+    if at is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device must run outside CUDA graph capture")
+        st = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        torch.cuda.synchronize(index)
+        _status[index] = st
+        at = _words[index] = st.data_ptr()
+    return at
 
 
 def read_status(clear: bool = True) -> int:
@@ -78,19 +84,47 @@ def ortho_options(coefficients, steps, eps, momentum=0.0, nesterov=False):
                                float(eps), float(momentum)), arr
 
 
+class _On:
+    """``with _On(index):`` the calls inside see that device as the current one."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.before)
+
+
+def _call(size_fn, fn, what, args, dev):
+    """One call of the library on the current stream of ``dev``: its workspace, sized by
+    ``size_fn``, is allocated on that stream, so it is reused only for work ordered after the
+    call."""
+    index = dev.index
+    with _On(index):
+        need = size_fn(*args)
+        if need == 0:
+            why = _lib.load().ta_last_error()
+            if why:
+                raise _lib.TurboAdamBackendError(
+                    f"{what} failed: {why.decode(errors='replace')}")
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = fn(*args, ws.data_ptr(), need, _word(index), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
+
+
 def run_ortho(table, n, options, dev):
     """One ta_orthogonalize call on the current stream of ``dev``."""
     lib = _lib.load()
-    need = lib.ta_ortho_workspace_size(table, n, ctypes.byref(options))
-    if need == 0 and lib.ta_last_error():
-        raise _lib.TurboAdamBackendError(
-            f"ta_ortho_workspace_size failed: {lib.ta_last_error().decode(errors='replace')}")
-    with torch.cuda.device(dev):
-        # allocated on the current stream: reused only for work ordered after this call
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        rc = lib.ta_orthogonalize(table, n, ctypes.byref(options), ws.data_ptr(), ws.numel(),
-                                  status_word(dev).data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc, "ta_orthogonalize")
+    _call(lib.ta_ortho_workspace_size, lib.ta_orthogonalize, "ta_orthogonalize",
+          (table, n, ctypes.byref(options)), dev)
 
 
 @torch.no_grad()
@@ -105,8 +139,8 @@ def orthogonalize(x: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
 
     The products take fp16 operands and fp32 sums. A 16-bit x enters
     unrounded, a 32-bit one as a pair of fp16 numbers; the result is within
-    about 1e-3 of the exact iteration (2-norm), so float32 outputs carry about
-    ten good bits. A zero matrix gives zero; a matrix with a NaN or an
+    about 1.5e-3 of the exact iteration (2-norm), so float32 outputs carry about
+    nine good bits. A zero matrix gives zero; a matrix with a NaN or an
     infinity gives NaN throughout. Not differentiable.
     """
     _lib.require_cuda(x)
@@ -147,48 +181,33 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if (c <= 1 or sc == 1) and (r <= 1 or sr >= c) else t.contiguous()
 
 
-def _strides(t):
-    return (ctypes.c_int64 * 2)(*t.stride())
-
-
-def _call_linear(fn_size, fn, what, op, dev):
-    lib = _lib.load()
-    need = fn_size(ctypes.byref(op))
-    if need == 0 and lib.ta_last_error():
-        raise _lib.TurboAdamBackendError(
-            f"{what} failed: {lib.ta_last_error().decode(errors='replace')}")
-    with torch.cuda.device(dev):
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        rc = fn(ctypes.byref(op), ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(),
-                _lib.stream_ptr(dev))
-    _lib.check(rc, what)
+# ta_linear and ta_linear_grad (include/turboadam_b200_matrix.h), packed in one go
+_LINEAR = struct.Struct("@6P3q2q2q2q4i")
+_LINEAR_GRAD = struct.Struct("@7P3qq2q2q2q2i")
 
 
 def _forward(x, w, bias, act, residual, need_deriv):
     lib = _lib.load()
     x, w = _two_strides(x), _two_strides(w)
-    tokens, fan_in, fan_out = x.shape[0], x.shape[1], w.shape[0]
-    y = torch.empty(tokens, fan_out, dtype=x.dtype, device=x.device)
+    (tokens, fan_in), fan_out = x.shape, w.shape[0]
+    dev = x.device
+    y = torch.empty((tokens, fan_out), dtype=x.dtype, device=dev)
     deriv = None
     if need_deriv:
-        deriv = torch.empty(tokens, (fan_out + 7) // 8 * 8, dtype=torch.int16, device=x.device)
-    op = _lib.TaLinear()
-    op.x_dev, op.w_dev, op.y_dev = x.data_ptr(), w.data_ptr(), y.data_ptr()
-    op.tokens, op.fan_in, op.fan_out = tokens, fan_in, fan_out
-    op.x_strides, op.w_strides = _strides(x), _strides(w)
-    op.y_stride = max(fan_out, 1)
-    op.dtype, op.activation = _DTYPES[x.dtype], act
+        deriv = torch.empty((tokens, (fan_out + 7) // 8 * 8), dtype=torch.int16, device=dev)
+    if tokens == 0 or fan_out == 0:
+        return y, deriv
     if bias is not None:
         bias = bias.contiguous()
-        op.bias_dev, op.bias_dtype = bias.data_ptr(), _DTYPES[bias.dtype]
     if residual is not None:
         residual = _rows(residual)
-        op.residual_dev, op.residual_stride = residual.data_ptr(), residual.stride(0)
-    if deriv is not None:
-        op.deriv_dev = deriv.data_ptr()
-    if y.numel():
-        _call_linear(lib.ta_linear_workspace_size, lib.ta_linear_forward, "ta_linear_forward", op,
-                     x.device)
+    op = _LINEAR.pack(
+        x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if residual is None else residual.data_ptr(), y.data_ptr(),
+        0 if deriv is None else deriv.data_ptr(), tokens, fan_in, fan_out, *x.stride(),
+        *w.stride(), 0 if residual is None else residual.stride(0), fan_out, _DTYPES[x.dtype],
+        0 if bias is None else _DTYPES[bias.dtype], act, 0)
+    _call(lib.ta_linear_workspace_size, lib.ta_linear_forward, "ta_linear_forward", (op,), dev)
     return y, deriv
 
 
@@ -196,13 +215,12 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act):
         # the derivative is needed by every gradient but the residual's
-        need = act != _lib.TA_ACT_NONE and any(ctx.needs_input_grad[:3])
+        nx, nw, nb, _, _ = ctx.needs_input_grad
+        need = act != _lib.TA_ACT_NONE and (nx or nw or nb)
         y, deriv = _forward(x, w, bias, act, residual, need)
-        ctx.act = act
         ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None,
-                              w if ctx.needs_input_grad[0] else None, deriv)
-        ctx.dims = (x.shape[0], x.shape[1], w.shape[0])
+        ctx.save_for_backward(x if nw else None, w if nx else None, deriv)
+        ctx.dims = (*x.shape, w.shape[0])
         # the weight's gradient is laid out as the weight: input by output if its rows are
         ctx.io = w.stride(0) == 1 and w.stride(1) != 1
         return y
@@ -210,37 +228,38 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, deriv = ctx.saved_tensors
-        tokens, fan_in, fan_out = ctx.dims
         nx, nw, nb, nr, _ = ctx.needs_input_grad
         dx = dw = db = None
         if nx or nw or nb:
             lib = _lib.load()
+            x, w, deriv = ctx.saved_tensors
+            tokens, fan_in, fan_out = ctx.dims
+            dev, dtype = dy.device, dy.dtype
             g = _rows(dy)
-            op = _lib.TaLinearGrad()
-            op.dy_dev, op.dy_stride = g.data_ptr(), max(g.stride(0), fan_out)
-            op.tokens, op.fan_in, op.fan_out = tokens, fan_in, fan_out
-            op.dtype = _DTYPES[dy.dtype]
-            if deriv is not None:
-                op.deriv_dev = deriv.data_ptr()
+            xs = ws = dws = (0, 0)
+            xp = wp = 0
             if nx:
                 w = _two_strides(w)
-                op.w_dev, op.w_strides = w.data_ptr(), _strides(w)
-                dx = torch.empty(tokens, fan_in, dtype=dy.dtype, device=dy.device)
-                op.dx_dev = dx.data_ptr()
+                wp, ws = w.data_ptr(), w.stride()
+                dx = torch.empty((tokens, fan_in), dtype=dtype, device=dev)
             if nw:
                 x = _two_strides(x)
-                op.x_dev, op.x_strides = x.data_ptr(), _strides(x)
+                xp, xs = x.data_ptr(), x.stride()
                 if ctx.io:
-                    dw = torch.empty(fan_in, fan_out, dtype=dy.dtype, device=dy.device).t()
+                    dw = torch.empty((fan_in, fan_out), dtype=dtype, device=dev).t()
                 else:
-                    dw = torch.empty(fan_out, fan_in, dtype=dy.dtype, device=dy.device)
-                op.dw_dev, op.dw_strides = dw.data_ptr(), _strides(dw)
+                    dw = torch.empty((fan_out, fan_in), dtype=dtype, device=dev)
+                dws = dw.stride()
             if nb:
-                db = torch.empty(fan_out, dtype=ctx.bias_dtype, device=dy.device)
-                op.db_dev, op.bias_dtype = db.data_ptr(), _DTYPES[db.dtype]
-            _call_linear(lib.ta_linear_backward_workspace_size, lib.ta_linear_backward,
-                         "ta_linear_backward", op, dy.device)
+                db = torch.empty(fan_out, dtype=ctx.bias_dtype, device=dev)
+            op = _LINEAR_GRAD.pack(
+                g.data_ptr(), 0 if deriv is None else deriv.data_ptr(), xp, wp,
+                0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                0 if db is None else db.data_ptr(), tokens, fan_in, fan_out,
+                max(g.stride(0), fan_out), *xs, *ws, *dws, _DTYPES[dtype],
+                0 if db is None else _DTYPES[db.dtype])
+            _call(lib.ta_linear_backward_workspace_size, lib.ta_linear_backward,
+                  "ta_linear_backward", (op,), dev)
         return dx, dw, db, dy if nr else None, None
 
 
@@ -261,8 +280,10 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     dz = dy * derivative is rounded once to the operand type for the two
     products that read it. A weight's gradient has the weight's layout.
     """
-    _lib.require_cuda(x)
-    if activation not in _ACTIVATIONS:
+    if not x.is_cuda:
+        _lib.require_cuda(x)
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(k for k in _ACTIVATIONS if k)} or "
                          f"None, got {activation!r}")
     if x.dtype not in _HALF:
@@ -270,22 +291,33 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match: "
                          "[..., fan_in] and [fan_out, fan_in] are wanted")
-    fan_out = weight.shape[0]
+    fan_in, fan_out = weight.shape[1], weight.shape[0]
     shape = (*x.shape[:-1], fan_out)
-    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is None:
-            continue
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-        if t.dtype != x.dtype and not (name == "bias" and t.dtype == torch.float32):
-            raise ValueError(f"{name} has dtype {t.dtype}, x has {x.dtype}")
-    if bias is not None and tuple(bias.shape) != (fan_out,):
-        raise ValueError(f"bias has shape {tuple(bias.shape)}, wanted {(fan_out,)}")
-    if residual is not None and tuple(residual.shape) != shape:
-        raise ValueError(f"residual has shape {tuple(residual.shape)}, wanted {shape}")
-    tokens = 1
-    for d in x.shape[:-1]:
-        tokens *= d
-    x2 = x.reshape(tokens, x.shape[-1])
-    r2 = None if residual is None else residual.reshape(tokens, fan_out)
-    return _LinearAct.apply(x2, weight, bias, r2, _ACTIVATIONS[activation]).reshape(shape)
+    dtype, device = x.dtype, x.device
+    if weight.dtype != dtype or weight.device != device:
+        raise ValueError(f"weight is {weight.dtype} on {weight.device}, x {dtype} on {device}")
+    grad = x.requires_grad or weight.requires_grad
+    if bias is not None:
+        if bias.device != device or (bias.dtype != dtype and bias.dtype != torch.float32):
+            raise ValueError(f"bias is {bias.dtype} on {bias.device}, x {dtype} on {device}")
+        if bias.dim() != 1 or bias.shape[0] != fan_out:
+            raise ValueError(f"bias has shape {tuple(bias.shape)}, wanted {(fan_out,)}")
+        grad = grad or bias.requires_grad
+    if residual is not None:
+        if residual.dtype != dtype or residual.device != device:
+            raise ValueError(f"residual is {residual.dtype} on {residual.device}, x {dtype} on "
+                             f"{device}")
+        if residual.shape != shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, wanted {shape}")
+        grad = grad or residual.requires_grad
+    flat = x.dim() == 2
+    if not flat:
+        tokens = math.prod(x.shape[:-1])
+        x = x.reshape(tokens, fan_in)
+        if residual is not None:
+            residual = residual.reshape(tokens, fan_out)
+    if grad and torch.is_grad_enabled():
+        y = _LinearAct.apply(x, weight, bias, residual, act)
+    else:
+        y, _ = _forward(x, weight, bias, act, residual, False)
+    return y if flat else y.reshape(shape)
