@@ -34,7 +34,7 @@ UNITS = {
         _paths("ta_kernels.cuh", "ta_codec.cuh", "ta_device.cuh", "ta_math.h", "ta_host.h")
         + [os.path.join(INCLUDE, "turboadam_b200.h")],
     os.path.join(HERE, "ta_mx_api.cu"):
-        _paths("ta_mx_device.cuh", "ta_mx_product.cuh", "ta_mx_elementwise.cuh", "ta_mx_few.cuh",
+        _paths("ta_mx_device.cuh", "ta_mx_product.cuh", "ta_mx_chain.cuh", "ta_mx_elementwise.cuh", "ta_mx_few.cuh",
                   "ta_host.h")
         + [os.path.join(INCLUDE, "turboadam_b200.h"),
            os.path.join(INCLUDE, "turboadam_b200_matrix.h")],

@@ -16,6 +16,7 @@
 
 #include "../../include/turboadam_b200_matrix.h"
 #include "ta_host.h"
+#include "ta_mx_chain.cuh"
 #include "ta_mx_elementwise.cuh"
 #include "ta_mx_few.cuh"
 #include "ta_mx_product.cuh"
@@ -44,6 +45,8 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline int64_t dt_bytes(int dt) { return dt == TA_F32 ? 4 : 2; }
 
 constexpr int64_t kMaxDim = 0x7fffff00;  // every dimension (rows, columns) is held in 32 bits
+
+constexpr int kMaxDevices = 64;
 
 int sm_count() {
   int dev = 0, n = 0;
@@ -95,31 +98,26 @@ struct Operand {
   const void* p = nullptr;
   int64_t mn = 0, k = 0, ld = 0, zs = 0, z = 1;
   bool mn_major = false;
+  bool sym = false;  // stored in its upper triangle of blocks
 };
 
-// The map one stage of an operand is loaded with: box_mn rows (or columns) of the output by 64
-// k's. *kind: 0 K-major; 1 MN-major, one copy for each chunk of 64; 2 MN-major in one copy, over
-// chunks as a dimension of their own, where the lines are whole chunks (a chunk that ran over the
-// end of a line would read the next one, and past the end of the last).
-ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn, int16_t* kind) {
+// How a stage of an operand is copied: 0 K-major; 1 MN-major, one copy for each chunk of 64;
+// 2 MN-major in one copy, over chunks as a dimension of their own, where the lines are whole
+// chunks (a chunk that ran over the end of a line would read the next one, and past the end of the
+// last).
+int kind_of(const Operand& o) { return !o.mn_major ? 0 : o.mn % 64 ? 1 : 2; }
+
+// The map of an operand whose stages hold box_mn rows (or columns) of the output by 64 k's.
+ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn) {
   EncodeFn fn = encode_fn();
   if (!fn) return ta_fail(TA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const cuuint64_t line = (cuuint64_t)o.ld * 2;
   const cuuint64_t plane = (cuuint64_t)std::max<int64_t>(o.zs, o.ld) * 2;
+  const int kind = kind_of(o);
   cuuint64_t dims[4], strides[3];
   cuuint32_t box[4] = {64, 64, 1, 1}, step[4] = {1, 1, 1, 1};
   cuuint32_t rank = 3;
-  if (!o.mn_major) {
-    *kind = 0;
-    dims[0] = (cuuint64_t)o.k;
-    dims[1] = (cuuint64_t)o.mn;
-    box[1] = (cuuint32_t)box_mn;
-  } else if (o.mn % 64) {
-    *kind = 1;
-    dims[0] = (cuuint64_t)o.mn;
-    dims[1] = (cuuint64_t)o.k;
-  } else {
-    *kind = 2;
+  if (kind == 2) {
     rank = 4;
     dims[0] = 64;
     dims[1] = (cuuint64_t)o.k;
@@ -129,11 +127,13 @@ ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn, int1
     strides[1] = 128;
     strides[2] = plane;
     box[2] = (cuuint32_t)(box_mn / 64);
-  }
-  if (rank == 3) {
+  } else {
+    dims[0] = (cuuint64_t)(kind == 0 ? o.k : o.mn);
+    dims[1] = (cuuint64_t)(kind == 0 ? o.mn : o.k);
     dims[2] = (cuuint64_t)o.z;
     strides[0] = line;
     strides[1] = plane;
+    if (kind == 0) box[1] = (cuuint32_t)box_mn;
   }
   CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   rank, const_cast<void*>(o.p), dims, strides, box, step,
@@ -144,16 +144,14 @@ ta_status make_map(CUtensorMap* m, const Operand& o, bool bf16, int box_mn, int1
   return TA_OK;
 }
 
-// ---- one launch of the tile engine -----------------------------------------------
+// ---- products on the tile engine ---------------------------------------------------
 struct Product {
   Operand a, b;
   int64_t M = 0, N = 0;
-  int parts = 1;
+  int parts = 1;        // operand pairs the sum runs over
   bool sym = false;
-  int64_t batch = 1;
   bool padded = false;  // the result's lines have room for whole chunks
-  Problem ep;           // the epilogue's fields
-  Product() { memset(&ep, 0, sizeof(ep)); }
+  int64_t batch = 1;
 };
 
 int64_t blocks_of(const Product& p) { return cdiv(p.a.k, kDepth) * p.parts; }
@@ -191,12 +189,17 @@ double tile_cycles(double kblocks, int cols) {
 // give every pair of SMs a share of a small result. Where even the narrow ones do not, long sums
 // are split: the partial tiles cost about 3000 cycles and a pass over them per split.
 Shape choose(const std::vector<Product>& ps, int pairs) {
-  bool b_mn = false;
-  for (const Product& p : ps) b_mn = b_mn || p.b.mn_major;
-  static const int kAny[] = {256, 224, 192, 160, 128, 96, 64};
-  static const int kChunked[] = {256, 128};  // a CTA's share is whole 64s
-  const int* widths = b_mn ? kChunked : kAny;
-  const int n_widths = b_mn ? 2 : 7;
+  // MN-major (or partly transposed) operands come in whole chunks of 64 rows a CTA; the tile widths
+  // of a symmetric result divide its blocks of 256
+  bool chunked = false, sym = false;
+  for (const Product& p : ps) {
+    chunked = chunked || p.b.mn_major || p.b.sym;
+    sym = sym || p.sym;
+  }
+  static const int kAny[] = {256, 224, 192, 160, 128, 96, 64}, kSym[] = {256, 128, 64},
+                   kChunked[] = {256, 128};
+  const int* widths = chunked ? kChunked : sym ? kSym : kAny;
+  const int n_widths = chunked ? 2 : sym ? 3 : 7;
   Shape best;
   best.splits.assign(ps.size(), 1);
   double best_time = 1e300;
@@ -269,20 +272,18 @@ ta_status launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
   return TA_OK;
 }
 
-// Shared-memory limit and resident pairs of an instance, found once per device. A die's SM count
-// need not divide into pairs, so the pairs that fit are asked for: one that had to wait for
-// another to finish would double the time of a persistent launch.
-template <int EPI, int DT>
-ta_status pairs_of(int* pairs) {
-  constexpr int kMaxDevices = 64;
+// Shared-memory limit and resident pairs of a kernel of the tile engine, found once per device. A
+// die's SM count need not divide into pairs, so the pairs that fit are asked for: one that had to
+// wait for another to finish would double the time of a persistent launch.
+template <typename Kernel>
+ta_status pairs_of(Kernel kernel, int* found, int* pairs) {  // found: [kMaxDevices], zero at first
   static std::mutex m;
-  static int found[kMaxDevices] = {};
   int dev = 0;
   MX_CU(cudaGetDevice(&dev));
   if (dev >= kMaxDevices) return ta_fail(TA_ERR_UNSUPPORTED, "device index over 63");
   std::lock_guard<std::mutex> lock(m);
   if (!found[dev]) {
-    MX_CU(cudaFuncSetAttribute(k_product<EPI, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    MX_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)kProductSmem));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
@@ -295,7 +296,7 @@ ta_status pairs_of(int* pairs) {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    MX_CU(cudaOccupancyMaxActiveClusters(&n, k_product<EPI, DT>, &cfg));
+    MX_CU(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
     if (n < 1) return ta_fail(TA_ERR_CUDA, "the product kernel does not fit this device");
     found[dev] = n;
   }
@@ -303,81 +304,76 @@ ta_status pairs_of(int* pairs) {
   return TA_OK;
 }
 
-template <int EPI, int DT>
-ta_status launch_product(const ProductArgs& g, int pairs, cudaStream_t stream) {
-  const unsigned grid = 2u * (unsigned)std::min<int64_t>(g.units, pairs);
-  return launch(k_product<EPI, DT>, dim3(grid), kThreads, kProductSmem, stream, g);
+// The device's view of a list of products of one tile width; returns the work units.
+int64_t place_products(const std::vector<Product>& ps, const Shape& shape, float* split_ws,
+                       uint32_t* split_count, Problem* out, int64_t* split_tiles) {
+  int64_t units = 0, floats = 0;
+  *split_tiles = 0;
+  for (size_t i = 0; i < ps.size(); ++i) {
+    const Product& p = ps[i];
+    Problem& P = out[i];
+    memset(&P, 0, sizeof(P));
+    P.M = (int32_t)p.M;
+    P.N = (int32_t)p.N;
+    P.n_end = (int32_t)(p.padded ? up32(p.N) : p.N);
+    P.kblocks = (int32_t)cdiv(p.a.k, kDepth);
+    P.tiles_m = (int32_t)cdiv(p.M, kTileRows);
+    P.tiles_n = (int32_t)cdiv(p.N, shape.cols);
+    P.tiles = (int32_t)tiles_of(p, shape.cols);
+    P.first = (int32_t)units;
+    P.batch = (int32_t)p.batch;
+    P.splits = shape.splits[i];
+    P.sym = p.sym;
+    P.a_kind = (int16_t)kind_of(p.a);
+    P.b_kind = (int16_t)kind_of(p.b);
+    P.a_sym = p.a.sym ? (int16_t)(p.a.mn % 64 ? 1 : 2) : 0;
+    P.b_sym = p.b.sym ? (int16_t)(p.b.mn % 64 ? 1 : 2) : 0;
+    const int64_t tiles = tiles_of(p, shape.cols) * p.batch;
+    if (P.splits > 1) {
+      P.split_ws = split_ws + floats;
+      P.split_count = split_count + *split_tiles;
+      floats += 2 * tiles * P.splits * kRows * shape.cols;
+      *split_tiles += 2 * tiles;
+    }
+    units += tiles * P.splits;
+  }
+  return units;
 }
 
-struct Scalars {
-  float alpha = 1.f, c0 = 0.f, c1 = 0.f, c2 = 0.f;
-  int unit_pow = 0;
-};
+int stages_of(int cols) {
+  return (int)std::min<size_t>(kMaxStages,
+                               kOperandSpace / (size_t)(kTileABytes + cols * kDepth));
+}
 
-// split_ws / split_count: kSplitFloats and kSplitTiles of them; the counters are zero, or `clear`ed
-// here where a launch splits its sums.
-template <int EPI, int DT = DT_F16>
-ta_status run_products(const std::vector<Product>& all, bool bf16, const Scalars& sc,
-                       float* split_ws, uint32_t* split_count, bool clear, uint32_t* status,
-                       cudaStream_t stream) {
-  for (size_t lo = 0; lo < all.size(); lo += kMaxProblems) {
-    const std::vector<Product> ps(all.begin() + lo,
-                                  all.begin() + std::min(all.size(), lo + kMaxProblems));
-    MX_OK(bind_device());
-    int pairs = 0;
-    MX_OK((pairs_of<EPI, DT>(&pairs)));
-    const Shape shape = choose(ps, pairs);
-    ProductArgs g;
-    memset(&g, 0, sizeof(g));
-    g.count = (int)ps.size();
-    g.bf16 = bf16;
-    g.alpha = sc.alpha;
-    g.c0 = sc.c0;
-    g.c1 = sc.c1;
-    g.c2 = sc.c2;
-    g.unit_pow = sc.unit_pow;
-    g.status = status;
-    g.cols = shape.cols;
-    g.stages = (int)std::min<size_t>(
-        kMaxStages, kOperandSpace / (size_t)(kTileABytes + shape.cols * kDepth));
-    int64_t units = 0, split_floats = 0, split_tiles = 0;
-    for (size_t i = 0; i < ps.size(); ++i) {
-      const Product& p = ps[i];
-      Problem& P = g.p[i];
-      P = p.ep;
-      if (p.a.k > 0) {
-        MX_OK(make_map(&P.ta, p.a, bf16, kRows, &P.a_mn));
-        MX_OK(make_map(&P.tb, p.b, bf16, g.cols / 2, &P.b_mn));
-      }
-      P.M = (int32_t)p.M;
-      P.N = (int32_t)p.N;
-      P.n_end = (int32_t)(p.padded ? up32(p.N) : p.N);
-      P.kblocks = (int32_t)cdiv(p.a.k, kDepth);
-      P.parts = p.parts;
-      P.tiles_m = (int32_t)cdiv(p.M, kTileRows);
-      P.tiles_n = (int32_t)cdiv(p.N, shape.cols);
-      P.tiles = (int32_t)tiles_of(p, shape.cols);
-      P.first = (int32_t)units;
-      P.batch = (int32_t)p.batch;
-      P.splits = shape.splits[i];
-      P.sym = p.sym;
-      const int64_t tiles = (int64_t)P.tiles * p.batch;
-      if (P.splits > 1) {
-        P.split_ws = split_ws + split_floats;
-        P.split_count = split_count + split_tiles;
-        split_floats += 2 * tiles * P.splits * kRows * shape.cols;
-        split_tiles += 2 * tiles;
-      }
-      units += tiles * P.splits;
-    }
-    if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
-    if (units == 0) continue;
-    if (clear && split_tiles)
-      MX_CU(cudaMemsetAsync(split_count, 0, split_tiles * sizeof(uint32_t), stream));
-    g.units = (int32_t)units;
-    MX_OK((launch_product<EPI, DT>(g, pairs, stream)));
+// One linear product. split_ws / split_count: kSplitFloats and kSplitTiles of them.
+template <bool EPILOGUE, int DT>
+ta_status run_linear(const Product& p, const Out& out, float* split_ws, uint32_t* split_count,
+                     uint32_t* status, cudaStream_t stream) {
+  static int found[kMaxDevices];
+  int pairs = 0;
+  MX_OK(bind_device());
+  MX_OK(pairs_of(k_linear<EPILOGUE, DT>, found, &pairs));
+  const std::vector<Product> ps(1, p);
+  const Shape shape = choose(ps, pairs);
+  LinearArgs g;
+  memset(&g, 0, sizeof(g));
+  int64_t split_tiles = 0;
+  const int64_t units = place_products(ps, shape, split_ws, split_count, &g.p, &split_tiles);
+  if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
+  if (units == 0) return TA_OK;
+  if (p.a.k > 0) {
+    MX_OK(make_map(&g.ta, p.a, DT == DT_BF16, kRows));
+    MX_OK(make_map(&g.tb, p.b, DT == DT_BF16, shape.cols / 2));
   }
-  return TA_OK;
+  g.out = out;
+  g.units = (int32_t)units;
+  g.cols = shape.cols;
+  g.stages = stages_of(shape.cols);
+  g.status = status;
+  if (split_tiles)
+    MX_CU(cudaMemsetAsync(split_count, 0, split_tiles * sizeof(uint32_t), stream));
+  return launch(k_linear<EPILOGUE, DT>, dim3(2u * (unsigned)std::min<int64_t>(units, pairs)),
+                kThreads, kProductSmem, stream, g);
 }
 
 // ---- orthogonalisation -----------------------------------------------------------
@@ -391,7 +387,7 @@ struct Class {  // matrices of one shape
   int64_t rows = 0, cols = 0, ld = 0, side = 0, lds = 0, count = 0;
   int first = 0;  // first table slot
   bool pair = false, tall = false;
-  __half *x0 = nullptr, *x1 = nullptr, *gram = nullptr, *poly = nullptr, *prod = nullptr;
+  __half *x0 = nullptr, *x1 = nullptr, *square[3] = {nullptr, nullptr, nullptr};
   int64_t xs() const { return rows * ld; }
   int64_t ss() const { return side * lds; }
 };
@@ -466,24 +462,203 @@ struct OrthoSpace {
   Scale* scale;
   double* partial;
   uint32_t* split_count;
+  uint32_t* chain;  // [chains][2]: arrivals, stop
   float* split_ws;
 };
+
+int chains_of(const OrthoPlan& plan) { return (int)cdiv((int64_t)plan.classes.size(), kMaxClasses); }
 
 OrthoSpace carve_ortho(OrthoPlan* plan, Arena* a) {
   OrthoSpace s;
   s.table = a->take<Item>(plan->items);
   s.scale = a->take<Scale>(plan->items);
   s.partial = a->take<double>(plan->chunks);
-  s.split_count = a->take<uint32_t>(kSplitTiles);
+  // cleared together: counters of split tiles, then two words of each chain
+  s.split_count = a->take<uint32_t>(kSplitTiles + 2 * chains_of(*plan));
+  s.chain = s.split_count ? s.split_count + kSplitTiles : nullptr;
   s.split_ws = a->take<float>(kSplitFloats);
   for (Class& c : plan->classes) {
     c.x0 = a->take<__half>(c.xs() * c.count * (c.pair ? 2 : 1));
     c.x1 = a->take<__half>(c.xs() * c.count);
-    c.gram = a->take<__half>(c.ss() * c.count);
-    c.poly = a->take<__half>(c.ss() * c.count);
-    c.prod = a->take<__half>(c.ss() * c.count);
+    for (__half*& q : c.square) q = a->take<__half>(c.ss() * c.count);
   }
   return s;
+}
+
+// Steps go in pairs. With A the Gram matrix of X, P and P' the polynomials of two steps,
+//   T = P A,  A' = P T  (the Gram matrix of P X, without forming P X),  Q = P' P,  X <- Q X:
+// in units of a side^3 product and with r = long / short side, 3 r + 5 for two steps against
+// 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the unrounded
+// input. Rounding A, and not X, costs accuracy where A's small eigenvalues drown in the error
+// of its large ones; over two steps (with the input exact) they do not: 1.3e-3 to 1.7e-3 of the
+// result on spectra that decay by 50 to 800, against 1.8e-3 to 2.6e-3 one by one (bf16
+// operands: 2e-2). Over three they would (1e-2).
+int chain_phases(const ta_ortho_options* o, Phase* out) {
+  int n = 0;
+  auto add = [&](int type, int end, int a, int b, int to, float alpha) -> Phase& {
+    Phase& p = out[n++];
+    memset(&p, 0, sizeof(p));
+    p.type = (int8_t)type;
+    p.end = (int8_t)end;
+    p.a = (int8_t)a;
+    p.b = (int8_t)b;
+    p.out = (int8_t)to;
+    p.alpha = alpha;
+    return p;
+  };
+  int x = BUF_X0, gram = BUF_S0, poly = BUF_S0 + 1, prod = BUF_S0 + 2;
+  auto polynomial = [&](int step) {
+    const double* abc = o->coefficients + 3 * step;
+    Phase& p = add(PH_SQUARE, END_POLY, gram, gram, poly,
+                   (float)(kScaleP * abc[2] / ((double)kScaleA * kScaleA)));
+    p.c0 = (float)(kScaleP * abc[0]);
+    p.c1 = (float)(kScaleP * abc[1] / kScaleA);
+    p.aux = (int8_t)gram;
+  };
+  for (int step = 0; step < o->steps;) {
+    const bool first = step == 0, two = step + 1 < o->steps;
+    add(PH_GRAM, END_SCALE, x, x, gram, first ? kScaleA : kScaleA / (kScaleX * kScaleX))
+        .unit_pow = first ? 2 : 0;
+    polynomial(step);
+    if (two) {
+      add(PH_SQUARE, END_SCALE, poly, gram, prod, kScaleT / (kScaleP * kScaleA));  // T
+      add(PH_SQUARE, END_SCALE, poly, prod, gram, kScaleA / (kScaleP * kScaleT));  // A'
+      std::swap(poly, prod);                                                       // P
+      polynomial(step + 1);                                                        // P'
+      add(PH_SQUARE, END_SCALE, poly, prod, gram, 1.f / kScaleP);                  // Q
+      std::swap(poly, gram);
+    }
+    step += two ? 2 : 1;
+    const bool last = step == o->steps;
+    const int to = x == BUF_X0 ? BUF_X1 : BUF_X0;
+    const float alpha = first ? 1.f / kScaleP : 1.f / (kScaleP * kScaleX);
+    Phase& p = add(PH_APPLY, last ? END_FINAL : END_SCALE, poly, x, to,
+                   last ? alpha : alpha * kScaleX);
+    p.unit_pow = first ? 1 : 0;
+    p.whole = first;
+    x = to;
+  }
+  return n;
+}
+
+ta_status run_chain(const std::vector<Class>& classes, const ta_ortho_options* o,
+                    const OrthoSpace& sp, uint32_t* words, uint32_t* status, cudaStream_t stream) {
+  static int found[kMaxDevices];
+  int pairs = 0;
+  MX_OK(bind_device());
+  MX_OK(pairs_of(k_chain, found, &pairs));
+  static thread_local ChainArgs g;  // some 20 KB
+  memset(&g, 0, sizeof(g));
+  g.classes = (int32_t)classes.size();
+  g.phases = chain_phases(o, g.phase);
+
+  auto square = [](const Class& c, int i, bool transposed = false) {
+    Operand q;
+    q.p = c.square[i];
+    q.mn = q.k = c.side;
+    q.ld = c.lds;
+    q.zs = c.ss();
+    q.z = c.count;
+    q.mn_major = transposed;
+    q.sym = !transposed;
+    return q;
+  };
+  // an iterate as an operand: rows x cols, row-major, so its columns are contiguous
+  auto iterate = [](const Class& c, int i, bool sum_over_rows) {
+    Operand q;
+    q.p = i == 0 ? c.x0 : c.x1;
+    q.mn = sum_over_rows ? c.cols : c.rows;
+    q.k = sum_over_rows ? c.rows : c.cols;
+    q.ld = c.ld;
+    q.zs = c.xs();
+    q.z = c.count * (i == 0 && c.pair ? 2 : 1);
+    q.mn_major = sum_over_rows;
+    return q;
+  };
+  std::vector<Product> lists[3];
+  for (const Class& c : classes) {
+    Product p;
+    p.batch = c.count;
+    p.sym = p.padded = true;
+    p.M = p.N = c.side;
+    p.a = p.b = iterate(c, 0, c.tall);
+    lists[PH_GRAM].push_back(p);
+    p.a = p.b = square(c, 0);
+    lists[PH_SQUARE].push_back(p);
+    p.sym = p.padded = false;
+    p.M = c.rows;
+    p.N = c.cols;
+    p.a = c.tall ? iterate(c, 0, false) : square(c, 0);
+    p.b = c.tall ? square(c, 0) : iterate(c, 0, true);
+    p.parts = c.pair ? 2 : 1;
+    lists[PH_APPLY].push_back(p);
+  }
+  int64_t most = 0;
+  int widest = 0;
+  for (int t = 0; t < 3; ++t) {
+    Shape shape = choose(lists[t], pairs);
+    // an application of the first iterate may sum over two parts, the others over one: no split
+    // is planned on parts that are not there
+    if (t == PH_APPLY) shape.splits.assign(classes.size(), 1);
+    int64_t split_tiles = 0;
+    const int64_t units =
+        place_products(lists[t], shape, sp.split_ws, sp.split_count, g.p[t], &split_tiles);
+    if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
+    g.units[t] = (int32_t)units;
+    g.cols[t] = shape.cols;
+    most = std::max(most, units);
+    widest = std::max(widest, shape.cols);
+  }
+  for (size_t i = 0; i < classes.size(); ++i) {
+    const Class& c = classes[i];
+    ChainClass& d = g.c[i];
+    for (int x = 0; x < 2; ++x) {
+      const Operand gram = iterate(c, x, c.tall), app = iterate(c, x, !c.tall);
+      MX_OK(make_map(&d.maps[MAP_GRAM_A + x], gram, false, kRows));
+      MX_OK(make_map(&d.maps[MAP_GRAM_B + x], gram, false, g.cols[PH_GRAM] / 2));
+      MX_OK(make_map(&d.maps[MAP_APPLY_X + x], app, false,
+                     c.tall ? kRows : g.cols[PH_APPLY] / 2));
+    }
+    for (int q = 0; q < 3; ++q) {
+      MX_OK(make_map(&d.maps[MAP_SQUARE_A + q], square(c, q), false, kRows));
+      MX_OK(make_map(&d.maps[MAP_SQUARE_B + q], square(c, q), false, g.cols[PH_SQUARE] / 2));
+      MX_OK(make_map(&d.maps[MAP_APPLY_S + q], square(c, q), false, g.cols[PH_APPLY] / 2));
+      MX_OK(make_map(&d.maps[MAP_SQUARE_A_T + q], square(c, q, true), false, kRows));
+      MX_OK(make_map(&d.maps[MAP_SQUARE_B_T + q], square(c, q, true), false,
+                     g.cols[PH_SQUARE] / 2));
+      MX_OK(make_map(&d.maps[MAP_APPLY_S_T + q], square(c, q, true), false,
+                     g.cols[PH_APPLY] / 2));
+      d.buf[BUF_S0 + q] = c.square[q];
+    }
+    d.buf[BUF_X0] = c.x0;
+    d.buf[BUF_X1] = c.x1;
+    d.xs = c.xs();
+    d.ss = c.ss();
+    d.ld = (int32_t)c.ld;
+    d.lds = (int32_t)c.lds;
+    d.tall = c.tall;
+    d.pair = c.pair;
+    d.scale = sp.scale + c.first;
+    d.items = sp.table + c.first;
+  }
+  g.stages = stages_of(widest);
+  g.stage_bytes = kTileABytes + widest * kDepth;
+  g.arrivals = words;
+  g.stop = words + 1;
+  g.status = status;
+
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeCooperative;
+  attr.val.cooperative = 1;
+  cfg.gridDim = dim3(2u * (unsigned)std::min<int64_t>(most, pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kProductSmem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  MX_CU(cudaLaunchKernelEx(&cfg, k_chain, g));
+  return TA_OK;
 }
 
 ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoPlan& plan,
@@ -534,7 +709,7 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
     ta.scale = sp.scale;
     ta.partial = sp.partial;
     ta.zero = sp.split_count;
-    ta.zero_words = lo == 0 ? (int32_t)kSplitTiles : 0;
+    ta.zero_words = lo == 0 ? (int32_t)kSplitTiles + 2 * chains_of(plan) : 0;
     int64_t most = 1;
     for (int i = 0; i < ta.count; ++i) most = std::max<int64_t>(most, ta.s[i].batch);
     MX_OK(launch(k_table, dim3((unsigned)std::min<int64_t>(cdiv(most, kEltThreads), 64)),
@@ -547,152 +722,11 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
   MX_OK(launch(k_scale, dim3((unsigned)chunk), kEltThreads, 0, stream, sp.table, items, mu,
                o->nesterov, o->eps));
 
-  const size_t nc = plan.classes.size();
-  auto square = [](const Class& c, const __half* p) {
-    Operand q;
-    q.p = p;
-    q.mn = q.k = c.side;
-    q.ld = c.lds;
-    q.zs = c.ss();
-    q.z = c.count;
-    return q;
-  };
-  // the iterate as an operand: rows x cols, row-major, so its columns are contiguous
-  auto iterate = [](const Class& c, const __half* p, bool sum_over_rows, int64_t z) {
-    Operand q;
-    q.p = p;
-    q.mn = sum_over_rows ? c.cols : c.rows;
-    q.k = sum_over_rows ? c.rows : c.cols;
-    q.ld = c.ld;
-    q.zs = c.xs();
-    q.z = z;
-    q.mn_major = sum_over_rows;
-    return q;
-  };
-  // A from X; the first iterate is x0 (its upper half, if a pair)
-  auto gram = [&](bool first) {
-    std::vector<Product> ps;
-    for (const Class& c : plan.classes) {
-      Product p;
-      const bool pair = c.pair && first;
-      p.a = iterate(c, first ? c.x0 : c.x1, c.tall, c.count * (pair ? 2 : 1));
-      p.b = p.a;
-      p.M = c.side;
-      p.N = c.side;
-      p.padded = true;
-      p.sym = true;
-      p.batch = c.count;
-      p.ep.za = p.ep.zb = pair ? 2 : 1;
-      p.ep.out = c.gram;
-      p.ep.out_zs = c.ss();
-      p.ep.ldo = (int32_t)c.lds;
-      p.ep.scale = sp.scale + c.first;
-      ps.push_back(p);
-    }
-    return ps;
-  };
-  // out = a b of side x side matrices that commute, so that it is symmetric too
-  using Square = __half* Class::*;
-  auto squares = [&](Square a, Square b, Square out) {
-    std::vector<Product> ps;
-    for (const Class& c : plan.classes) {
-      Product p;
-      p.a = square(c, c.*a);
-      p.b = square(c, c.*b);
-      p.M = c.side;
-      p.N = c.side;
-      p.padded = true;
-      p.sym = true;
-      p.batch = c.count;
-      p.ep.za = p.ep.zb = 1;
-      p.ep.out = c.*out;
-      p.ep.out_zs = c.ss();
-      p.ep.ldo = (int32_t)c.lds;
-      p.ep.aux = c.*a;
-      p.ep.aux_zs = c.ss();
-      p.ep.ld_aux = (int32_t)c.lds;
-      p.ep.scale = sp.scale + c.first;
-      ps.push_back(p);
-    }
-    return ps;
-  };
-  // X <- poly * x (x * poly, if tall); from_x0: x is the scaled input, with both parts of a pair
-  // if `whole`
-  auto apply = [&](Square poly, bool first) {
-    std::vector<Product> ps;
-    for (const Class& c : plan.classes) {
-      Product p;
-      const bool pair = c.pair && first;
-      const Operand q = square(c, c.*poly);
-      const Operand v = iterate(c, first ? c.x0 : c.x1, !c.tall, c.count * (pair ? 2 : 1));
-      p.a = c.tall ? v : q;
-      p.b = c.tall ? q : v;
-      p.parts = pair ? 2 : 1;
-      p.M = c.rows;
-      p.N = c.cols;
-      p.batch = c.count;
-      p.ep.za = c.tall && pair ? 2 : 1;
-      p.ep.zb = !c.tall && pair ? 2 : 1;
-      p.ep.out = first ? c.x1 : c.x0;
-      p.ep.out_zs = c.xs();
-      p.ep.ldo = (int32_t)c.ld;
-      p.ep.scale = sp.scale + c.first;
-      p.ep.items = sp.table + c.first;
-      ps.push_back(p);
-    }
-    return ps;
-  };
-
-  // Steps go in pairs. With A the Gram matrix of X, P and P' the polynomials of two steps,
-  //   T = P A,  A' = P T  (the Gram matrix of P X, without forming P X),  Q = P' P,  X <- Q X:
-  // in units of a side^3 product and with r = long / short side, 3 r + 5 for two steps against
-  // 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the unrounded
-  // input. Rounding A, and not X, costs accuracy where A's small eigenvalues drown in the error
-  // of its large ones; over two steps (with the input exact) they do not: 1.3e-3 to 1.7e-3 of the
-  // result on spectra that decay by 50 to 800, against 1.8e-3 to 2.6e-3 one by one (bf16
-  // operands: 2e-2). Over three they would (1e-2).
-  auto run = [&](auto fn, const std::vector<Product>& ps, float alpha, int unit_pow) {
-    Scalars sc;
-    sc.alpha = alpha;
-    sc.unit_pow = unit_pow;
-    return fn(ps, false, sc, sp.split_ws, sp.split_count, false, status, stream);
-  };
-  auto polynomial = [&](int step) {
-    const double* abc = o->coefficients + 3 * step;
-    Scalars sc;
-    sc.c0 = (float)(kScaleP * abc[0]);
-    sc.c1 = (float)(kScaleP * abc[1] / kScaleA);
-    sc.c2 = (float)(kScaleP * abc[2] / ((double)kScaleA * kScaleA));
-    return run_products<EPI_POLY>(squares(&Class::gram, &Class::gram, &Class::poly), false, sc,
-                                  sp.split_ws, sp.split_count, false, status, stream);
-  };
-  for (int step = 0; step < o->steps;) {
-    const bool first = step == 0, two = step + 1 < o->steps;
-    MX_OK(run(run_products<EPI_GRAM>, gram(first),
-              first ? kScaleA : kScaleA / (kScaleX * kScaleX), first ? 2 : 0));
-    MX_OK(polynomial(step));
-    if (two) {
-      MX_OK(run(run_products<EPI_GRAM>, squares(&Class::poly, &Class::gram, &Class::prod),
-                kScaleT / (kScaleP * kScaleA), 0));
-      MX_OK(run(run_products<EPI_GRAM>, squares(&Class::poly, &Class::prod, &Class::gram),
-                kScaleA / (kScaleP * kScaleT), 0));
-      for (Class& c : plan.classes) std::swap(c.poly, c.prod);  // P
-      MX_OK(polynomial(step + 1));                              // P'
-      MX_OK(run(run_products<EPI_GRAM>, squares(&Class::poly, &Class::prod, &Class::gram),
-                1.f / kScaleP, 0));
-      for (Class& c : plan.classes) std::swap(c.poly, c.gram);  // Q
-    }
-    step += two ? 2 : 1;
-    const float alpha = first ? 1.f / kScaleP : 1.f / (kScaleP * kScaleX);
-    if (step == o->steps) {
-      MX_OK(run(run_products<EPI_FINAL>, apply(&Class::poly, first), alpha, first ? 1 : 0));
-    } else {
-      MX_OK(run(run_products<EPI_APPLY>, apply(&Class::poly, first), alpha * kScaleX,
-                first ? 1 : 0));
-      // the iterate is in x1 from now on; x0 takes the next one
-      if (!first)
-        for (Class& c : plan.classes) std::swap(c.x0, c.x1);
-    }
+  for (int i = 0; i < chains_of(plan); ++i) {
+    const size_t lo = (size_t)i * kMaxClasses;
+    const std::vector<Class> part(plan.classes.begin() + lo,
+                                  plan.classes.begin() + std::min(plan.classes.size(), lo + kMaxClasses));
+    MX_OK(run_chain(part, o, sp, sp.chain + 2 * i, status, stream));
   }
   return TA_OK;
 }
@@ -825,7 +859,8 @@ ta_status launch_few(FewArgs& g, bool cols, int64_t room, cudaStream_t stream) {
 }
 
 template <int DT>
-ta_status run_few(const Product& p, float* part, int64_t room, cudaStream_t stream) {
+ta_status run_few(const Product& p, const Out& out, float* part, int64_t room,
+                  cudaStream_t stream) {
   FewArgs g;
   memset(&g, 0, sizeof(g));
   g.a = reinterpret_cast<const uint16_t*>(p.a.p);
@@ -836,15 +871,15 @@ ta_status run_few(const Product& p, float* part, int64_t room, cudaStream_t stre
   g.N = (int)p.N;
   g.K = (int)p.a.k;
   g.part = part;
-  g.out = reinterpret_cast<uint16_t*>(p.ep.out);
-  g.aux = reinterpret_cast<const uint16_t*>(p.ep.aux);
-  g.bias = p.ep.bias;
-  g.deriv = p.ep.deriv;
-  g.ldo = p.ep.ldo;
-  g.ld_aux = p.ep.ld_aux;
-  g.ld_deriv = p.ep.ld_deriv;
-  g.bias_dt = p.ep.bias_dt;
-  g.act = p.ep.act;
+  g.out = reinterpret_cast<uint16_t*>(out.out);
+  g.aux = reinterpret_cast<const uint16_t*>(out.aux);
+  g.bias = out.bias;
+  g.deriv = out.deriv;
+  g.ldo = out.ld;
+  g.ld_aux = out.ld_aux;
+  g.ld_deriv = out.ld_deriv;
+  g.bias_dt = out.bias_dt;
+  g.act = out.act;
   const bool cols = p.b.mn_major;
   if (g.tokens == 1) return launch_few<DT, 1>(g, cols, room, stream);
   if (g.tokens == 2) return launch_few<DT, 2>(g, cols, room, stream);
@@ -853,18 +888,14 @@ ta_status run_few(const Product& p, float* part, int64_t room, cudaStream_t stre
 }
 
 // The products of one linear call: counters are cleared where a launch may split its sums.
-ta_status plain_product(const Product& p, bool bf16, const LinearSpace& s, uint32_t* status,
-                        cudaStream_t stream, bool linear) {
+ta_status plain_product(const Product& p, const Out& out, bool bf16, const LinearSpace& s,
+                        uint32_t* status, cudaStream_t stream, bool epilogue) {
   if (few_rows(p) && p.M * p.N <= kSplitFloats)
-    return bf16 ? run_few<DT_BF16>(p, s.split_ws, kSplitFloats, stream)
-                : run_few<DT_F16>(p, s.split_ws, kSplitFloats, stream);
-  const std::vector<Product> ps(1, p);
-  auto run = [&](auto fn) {
-    return fn(ps, bf16, Scalars(), s.split_ws, s.split_count, true, status, stream);
-  };
-  if (linear)
-    return bf16 ? run(run_products<EPI_LINEAR, DT_BF16>) : run(run_products<EPI_LINEAR, DT_F16>);
-  return bf16 ? run(run_products<EPI_PLAIN, DT_BF16>) : run(run_products<EPI_PLAIN, DT_F16>);
+    return bf16 ? run_few<DT_BF16>(p, out, s.split_ws, kSplitFloats, stream)
+                : run_few<DT_F16>(p, out, s.split_ws, kSplitFloats, stream);
+  auto run = [&](auto fn) { return fn(p, out, s.split_ws, s.split_count, status, stream); };
+  if (epilogue) return bf16 ? run(run_linear<true, DT_BF16>) : run(run_linear<true, DT_F16>);
+  return bf16 ? run(run_linear<false, DT_BF16>) : run(run_linear<false, DT_F16>);
 }
 
 struct GradLines {
@@ -1005,17 +1036,18 @@ ta_status ta_linear_forward(const ta_linear* op, void* workspace_dev, size_t wor
     }
     p.M = op->tokens;
     p.N = op->fan_out;
-    p.ep.za = p.ep.zb = 1;
-    p.ep.out = op->y_dev;
-    p.ep.ldo = (int32_t)op->y_stride;
-    p.ep.aux = op->residual_dev;
-    p.ep.ld_aux = (int32_t)op->residual_stride;
-    p.ep.bias = op->bias_dev;
-    p.ep.bias_dt = (int16_t)op->bias_dtype;
-    p.ep.act = (int16_t)op->activation;
-    p.ep.deriv = op->deriv_dev;
-    p.ep.ld_deriv = (int32_t)up8(op->fan_out);
-    return plain_product(p, op->dtype == TA_BF16, s, status_dev, stream, true);
+    Out out;
+    memset(&out, 0, sizeof(out));
+    out.out = reinterpret_cast<uint8_t*>(op->y_dev);
+    out.ld = op->y_stride;
+    out.aux = reinterpret_cast<const uint8_t*>(op->residual_dev);
+    out.ld_aux = op->residual_stride;
+    out.bias = op->bias_dev;
+    out.bias_dt = op->bias_dtype;
+    out.act = op->activation;
+    out.deriv = op->deriv_dev;
+    out.ld_deriv = up8(op->fan_out);
+    return plain_product(p, out, op->dtype == TA_BF16, s, status_dev, stream, true);
   } catch (const std::exception& e) {
     return ta_fail(TA_ERR_INVALID, e.what());
   }
@@ -1061,6 +1093,13 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
         MX_OK(launch(k_bias_grad, dim3((unsigned)cdiv(O, kEltThreads)), kEltThreads, 0, stream,
                      s.part, (int)g.row_parts, (int)O, op->db_dev, (int)op->bias_dtype));
     }
+    auto result = [](void* p, int64_t ld) {
+      Out out;
+      memset(&out, 0, sizeof(out));
+      out.out = reinterpret_cast<uint8_t*>(p);
+      out.ld = ld;
+      return out;
+    };
     auto dz_operand = [&](bool over_tokens) {  // summed over tokens (dw) or fan_out (dx)
       Operand o;
       o.p = dz;
@@ -1079,10 +1118,7 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
       }
       p.M = T;
       p.N = I;
-      p.ep.za = p.ep.zb = 1;
-        p.ep.out = op->dx_dev;
-      p.ep.ldo = (int32_t)I;
-      MX_OK(plain_product(p, bf16, s.lin, status_dev, stream, false));
+      MX_OK(plain_product(p, result(op->dx_dev, I), bf16, s.lin, status_dev, stream, false));
     }
     if (op->dw_dev && O > 0 && I > 0) {
       Product p;
@@ -1096,12 +1132,8 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
       p.M = g.dw_io ? I : O;
       p.N = g.dw_io ? O : I;
       const int64_t ldo = op->dw_strides[g.dw_io ? 1 : 0];
-      if (p.M > 1 && ldo > kMaxDim)
-        return ta_fail(TA_ERR_UNSUPPORTED, "a row stride is over 2^31 - 256");
-      p.ep.za = p.ep.zb = 1;
-        p.ep.out = op->dw_dev;
-      p.ep.ldo = (int32_t)(p.M > 1 ? ldo : p.N);
-      MX_OK(plain_product(p, bf16, s.lin, status_dev, stream, false));
+      MX_OK(plain_product(p, result(op->dw_dev, p.M > 1 ? ldo : p.N), bf16, s.lin, status_dev,
+                          stream, false));
     }
     return TA_OK;
   } catch (const std::exception& e) {

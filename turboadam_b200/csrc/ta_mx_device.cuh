@@ -97,17 +97,15 @@ __device__ __forceinline__ void cluster_sync_all() {
           : "memory");
 }
 
-// ---- mbarriers -------------------------------------------------------------
-__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count)
-               : "memory");
+// ---- mbarriers (by shared address) -----------------------------------------------
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(count) : "memory");
 }
 __device__ __forceinline__ void bar_init_fence() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
-__device__ __forceinline__ void bar_expect_tx(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)),
-               "r"(bytes)
+__device__ __forceinline__ void bar_expect_tx(uint32_t b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes)
                : "memory");
 }
 // Arrive on a barrier of any CTA of the cluster (shared::cluster address). What it orders is the
@@ -116,28 +114,31 @@ __device__ __forceinline__ void bar_expect_tx(uint64_t* b, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-__device__ __forceinline__ uint32_t bar_try(uint64_t* b, uint32_t parity) {
+__device__ __forceinline__ uint32_t bar_try(uint32_t b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_addr(b)), "r"(parity)
+      : "r"(b), "r"(parity), "r"(1000000u)  // may sleep for a millisecond
       : "memory");
   return ok;
 }
 // A wait that ends: false once kWaitLimitNs have passed, with the status bit set.
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, uint32_t* status) {
-  if (bar_try(b, parity)) return true;
+static __device__ __noinline__ bool bar_wait_on(uint32_t b, uint32_t parity, uint32_t* status) {
   const uint64_t t0 = now_ns();
   for (;;) {
-    if (bar_try(b, parity)) return true;
+    for (int i = 0; i < 16; ++i)
+      if (bar_try(b, parity)) return true;
     if (now_ns() - t0 > kWaitLimitNs) {
       atomicOr(status, kStatusTimeout);
       return false;
     }
   }
+}
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, uint32_t* status) {
+  return bar_try(b, parity) || bar_wait_on(b, parity, status);
 }
 
 // ---- TMA -------------------------------------------------------------------
@@ -165,9 +166,8 @@ __device__ __forceinline__ void tma_load4(const CUtensorMap* m, uint32_t dst, ui
 }
 
 // ---- tcgen05 (pairs of SMs) ----------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_addr(slot)),
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
                "r"(cols)
                : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -192,10 +192,10 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 }
 // Arrive on the barrier at `bar`'s offset in both CTAs of the pair when every matrix instruction
 // issued so far by this thread has finished.
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-      "[%0], %1;" ::"r"(smem_addr(bar)),
+      "[%0], %1;" ::"r"(bar),
       "h"((uint16_t)3)
       : "memory");
 }

@@ -14,13 +14,12 @@
 // give every pair of SMs a share of a small result. Two accumulators let a tile's epilogue run
 // under the next tile's products.
 //
-// Roles of the 19 warps: warps 0 and 1 issue the TMA loads of A and of B, warp 2
-// (of the pair's first CTA) the matrix instructions, warps 3..18 are the
-// epilogue, four to each 32-row quadrant of tensor memory. They take the tile's
-// 32-column chunks in turn and pass them through shared memory, so that every
-// global access covers whole sectors of consecutive lines. An epilogue chunk is
-// a chain of dependent instructions, some 1500 cycles: sixteen warps rather than
-// eight hide twice as much of it.
+// Roles of the 16 warps: warps 0 and 1 issue the TMA loads of A and of B, warp 2
+// (of the pair's first CTA) the matrix instructions, warp 3 rests, warps 4..15
+// are the epilogue, three to each 32-row quadrant of tensor memory. They take the
+// tile's 32-column chunks in turn and pass them through shared memory, so that
+// every global access covers whole sectors of consecutive lines. Twelve warps
+// leave each thread 128 registers; sixteen left 96, and spilled.
 //
 // Long sums with few tiles (the Gram matrix of a wide matrix; few tokens) are
 // split over k: each split leaves its fp32 tile in the workspace, and the last
@@ -40,25 +39,16 @@ constexpr int kTileRows = 256;  // rows of a pair's tile
 constexpr int kDepth = 64;      // k's per stage: one 128-byte swizzled row
 constexpr int kTileABytes = kRows * kDepth * 2;
 constexpr int kMaxStages = 8;
-constexpr int kFirstEpi = 3;  // first epilogue warp
-constexpr int kEpiWarps = 16;
+constexpr int kFirstEpi = 4;  // first epilogue warp
+constexpr int kTurns = 2;     // epilogue warps of a quadrant
+constexpr int kEpiWarps = 4 * kTurns;
+constexpr int kEpiStep = 32 * kTurns;  // a warp's chunks are this many columns apart
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kTmemCols = 512;
-constexpr int kMaxProblems = 8;  // per launch (they travel as kernel parameters)
 constexpr int kLine = 64;                   // bytes of a line of an epilogue block
 constexpr int kBlockBytes = 32 * kLine;     // per epilogue warp
 constexpr size_t kOperandSpace = 192 * 1024;
 constexpr size_t kProductSmem = 1024 + kOperandSpace + kEpiWarps * kBlockBytes + 256;
-
-// What is done with a finished tile.
-enum Epilogue {
-  EPI_GRAM = 0,   // fp16, symmetric: alpha * acc, mirrored
-  EPI_POLY = 1,   // fp16, symmetric: c0 I + c1 A + c2 acc (A read back), mirrored
-  EPI_APPLY = 2,  // fp16: alpha * acc
-  EPI_FINAL = 3,  // the orthogonalised update: stored, or applied to the parameter
-  EPI_LINEAR = 4, // bias, activation (and its derivative), residual
-  EPI_PLAIN = 5   // rounded to the output's type
-};
 
 // Per-matrix scale of a Newton-Schulz list: the stored fp16 input times `unit` is the
 // normalised matrix (unit is NaN where the input holds a NaN or an infinity).
@@ -85,61 +75,42 @@ struct Item {
   int16_t g_dt, mom_dt, out_dt, update;
 };
 
-struct alignas(64) Problem {
-  CUtensorMap ta, tb;
+// One product D[m][n] = sum_k A[m][k] B[n][k] of a launch, or of a phase of a chain: `batch`
+// independent ones of one shape.
+struct Problem {
   int32_t M, N;
   int32_t n_end;            // columns the epilogue writes: N, or whole chunks of padded lines
   int32_t kblocks;          // blocks of 64 k's in one part of the sum
-  int32_t parts;            // the sum runs over this many operand pairs
   int32_t tiles_m, tiles_n, tiles;  // per matrix (tiles: on and above the diagonal, if sym)
   int32_t first;            // first work unit of this problem in the launch
   int32_t batch, splits;
-  int32_t za, zb;           // z coordinate of (matrix z, part p): z * za + p * (za > 1)
-  int16_t a_mn, b_mn;       // 0: K-major; 1: MN-major, 64 at a time; 2: MN-major in one copy
-  int16_t sym, pad0;
-  int32_t ldo, ld_aux;
-  void* out;
-  int64_t out_zs;           // elements between matrices
-  const void* aux;          // EPI_POLY: A; EPI_LINEAR: residual
-  int64_t aux_zs;
-  const Scale* scale;       // [batch]
-  const Item* items;        // [batch] (EPI_FINAL)
-  const void* bias;         // EPI_LINEAR
-  int16_t* deriv;           // EPI_LINEAR: the activation's derivative, 2^-14 steps
-  int32_t ld_deriv;
-  int16_t bias_dt, act;
+  int16_t a_kind, b_kind;   // 0: K-major; 1: MN-major, 64 at a time; 2: MN-major in one copy
+  int16_t sym;              // the result is symmetric
+  int16_t a_sym, b_sym;     // the operand is (K-major; 1 or 2 of the kinds where transposed)
+  int16_t pad0;
   float* split_ws;          // [unit / splits][splits][rows x columns of a CTA tile]
   uint32_t* split_count;    // zero before and after every launch
-};
-
-struct ProductArgs {
-  Problem p[kMaxProblems];
-  int32_t count;
-  int32_t units;            // work units: tiles x matrices x splits, over all problems
-  int32_t bf16;             // operand type (all problems of a launch)
-  int32_t cols;             // tile width C
-  int32_t stages;
-  int32_t unit_pow;         // scale.unit enters alpha to this power (0, 1 or 2)
-  float alpha, c0, c1, c2;
-  uint32_t* status;
 };
 
 struct Unit {
   int p, z, m0, n0, split;
 };
 
-// First tile column of tile row i of a symmetric result: the one that holds the diagonal block's
-// first column. Columns left of the diagonal block are skipped by the epilogue, those right of it
-// are mirrored, in chunks of 32 columns (which divides 256 and every tile width).
+// A symmetric matrix is computed and stored in its upper triangle of 256 x 256 blocks only: row r
+// from column r & ~255 on. Tile row i of a symmetric result starts at tile column sym_first (tile
+// widths divide 256). As an operand, a block of k's left of the rows' diagonal block is read
+// transposed: the element (r, k) at (k, r), MN-major where the rest of the operand is K-major.
 __host__ __device__ __forceinline__ int sym_first(int i, int cols) { return i * kTileRows / cols; }
 
 // Work unit u of the launch. Tiles of a general product run down groups of 8 tile rows, so that
 // the CTAs in flight share operand tiles in L2; splits of one tile are neighbours.
-__device__ __forceinline__ Unit locate(const ProductArgs& g, int u, int p_hint) {
+template <class View>
+__device__ __forceinline__ Unit locate(const View& v, int u, int p_hint) {
   Unit w;
   int p = p_hint;
-  while (p + 1 < g.count && u >= g.p[p + 1].first) ++p;
-  const Problem& P = g.p[p];
+  while (p + 1 < v.count() && u >= v.problem(p + 1).first) ++p;
+  const Problem& P = v.problem(p);
+  const int cols = v.cols();
   w.p = p;
   int t = u - P.first;
   w.split = w.z = 0;
@@ -155,12 +126,12 @@ __device__ __forceinline__ Unit locate(const ProductArgs& g, int u, int p_hint) 
   if (P.sym) {
     i = 0;
     for (;;) {
-      const int n = P.tiles_n - sym_first(i, g.cols);
+      const int n = P.tiles_n - sym_first(i, cols);
       if (t < n) break;
       t -= n;
       ++i;
     }
-    j = sym_first(i, g.cols) + t;
+    j = sym_first(i, cols) + t;
   } else {
     int g0 = 0, rows = P.tiles_m;
     if (rows > 8) {
@@ -173,13 +144,14 @@ __device__ __forceinline__ Unit locate(const ProductArgs& g, int u, int p_hint) 
     i = g0 + t - j * rows;
   }
   w.m0 = i * kTileRows;
-  w.n0 = j * g.cols;
+  w.n0 = j * cols;
   return w;
 }
 
 // K blocks [*k0, *k1) of a split. (At most 32 splits of at most 2^25 blocks: 32 bits suffice.)
-__device__ __forceinline__ void split_range(const Problem& P, int split, int* k0, int* k1) {
-  const uint32_t total = (uint32_t)(P.kblocks * P.parts);
+__device__ __forceinline__ void split_range(const Problem& P, int parts, int split, int* k0,
+                                            int* k1) {
+  const uint32_t total = (uint32_t)(P.kblocks * parts);
   *k0 = 0;
   *k1 = (int)total;
   if (P.splits > 1) {
@@ -384,7 +356,7 @@ __device__ __forceinline__ void take_sums(const Sums& a, int c, float (&v)[32]) 
   }
 }
 
-// What the epilogue reads of a tile's problem, in registers.
+// Where a tile goes, and what its epilogue reads.
 struct Out {
   uint8_t* out;
   const uint8_t* aux;
@@ -393,6 +365,10 @@ struct Out {
   int64_t ld, ld_aux, ld_deriv;
   int bias_dt, act;
 };
+
+__device__ __forceinline__ void epilogue_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+}
 
 // A chunk of the orthogonalised update, stored or applied to the parameter.
 template <int DT>
@@ -474,296 +450,396 @@ __device__ __forceinline__ void finish_linear(const Out& o, const Block& b, floa
   block_store<2>(b, o.out + (row0 * o.ld + col) * 2, o.ld, n);
 }
 
-// One chunk: the sums of rows [row0, row0 + 32) by columns [col, col + n) of the result. DT is
-// the type of the result (EPI_LINEAR, EPI_PLAIN); `mirror`: a symmetric result's chunk right of
-// the diagonal block, also written transposed (a warp's 32 rows are 64 consecutive bytes).
-template <int EPI, int DT>
-__device__ __forceinline__ void finish(const ProductArgs& g, const Out& o, const Item* it,
-                                       const Block& b, float (&v)[32], float alpha, int64_t row0,
-                                       int col, int n, bool mirror, int N) {
-  if constexpr (EPI == EPI_GRAM || EPI == EPI_POLY || EPI == EPI_APPLY) {
-    if constexpr (EPI == EPI_POLY) {
-      block_load<2>(b, o.aux + (row0 * o.ld_aux + col) * 2, o.ld_aux, n);
-      const int diag = (int)row0 + b.lane - col;
-      row_get<DT_F16>(b, [&](int i, float x) {
-        v[i] = fmaf(g.c2, v[i], fmaf(g.c1, x, diag == i ? g.c0 : 0.f));
-      });
-    } else {
+// One chunk of a Newton-Schulz matrix: the sums v of rows [row0, row0 + 32) by columns
+// [col, col + n), stored in fp16 as alpha v, or as the polynomial c0 I + c1 A + alpha v of A = aux.
+template <bool POLY>
+__device__ __forceinline__ void finish_half(uint8_t* out, int64_t ld, const uint8_t* aux,
+                                            int64_t ld_aux, const Block& b, float (&v)[32],
+                                            float alpha, float c0, float c1, int64_t row0, int col,
+                                            int n) {
+  if constexpr (POLY) {
+    block_load<2>(b, aux + (row0 * ld_aux + col) * 2, ld_aux, n);
+    row_get<DT_F16>(b, [&](int i, float x) { v[i] = fmaf(alpha, v[i], c1 * x); });
+    if (row0 == col) {  // both are multiples of 32: the diagonal is in this chunk or not
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= alpha;
+      for (int i = 0; i < 32; ++i) v[i] += b.lane == i ? c0 : 0.f;
     }
-    row_put<DT_F16>(b, v);
-    if (EPI != EPI_APPLY && mirror && b.lane < b.rows) {
-      __half* t = reinterpret_cast<__half*>(o.out) + col * o.ld + row0 + b.lane;
-#pragma unroll
-      for (int i = 0; i < 32; ++i, t += o.ld)
-        if (i < N - col) *t = __float2half_rn(v[i]);  // n may run into the lines' padding
-    }
-    block_store<2>(b, o.out + (row0 * o.ld + col) * 2, o.ld, n);
-  } else if constexpr (EPI == EPI_FINAL) {
-    const int dt = it->out_dt;
-    if (dt == DT_BF16) finish_final<DT_BF16>(*it, b, v, alpha, N, row0, col, n);
-    else if (dt == DT_F32) finish_final<DT_F32>(*it, b, v, alpha, N, row0, col, n);
-    else finish_final<DT_F16>(*it, b, v, alpha, N, row0, col, n);
-  } else if constexpr (EPI == EPI_LINEAR) {
-    finish_linear<DT>(o, b, v, row0, col, n);
   } else {
-    row_put<DT>(b, v);
-    block_store<2>(b, o.out + (row0 * o.ld + col) * 2, o.ld, n);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= alpha;
+  }
+  row_put<DT_F16>(b, v);
+  block_store<2>(b, out + (row0 * ld + col) * 2, ld, n);
+}
+
+// ---- roles -----------------------------------------------------------------------
+// A CTA's shared-memory layout and place in the launch.
+struct Cta {
+  uint32_t tiles0;          // shared address of the operand stages
+  uint32_t full, empty;     // barriers, [kMaxStages] each
+  uint32_t acc_full, acc_empty;  // [2]
+  uint32_t last_flag;
+  uint32_t tmem;
+  uint32_t rank;            // in the pair
+  int worker, workers;      // this pair, pairs
+  int stages;
+  uint32_t stage_bytes;
+  uint32_t* status;
+};
+
+// Where a copy warp or the matrix warp stands in the ring of stages.
+struct Ring {
+  uint32_t count = 0;  // stages filled (or tiles computed) so far
+  int s = 0;
+  uint32_t phase;
+  bool ok = true;      // false once a wait has run out
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// Each role looks up its first unit, then passes `gate` (once, units or not), then touches memory:
+// what comes before (some 1500 cycles of parameters and index arithmetic) runs while the kernel or
+// phase before drains. gate() returns false if its wait ran out.
+
+// Warp 0 (A) or 1 (B): the loads of this pair's units. Both CTAs' bytes are counted on the first
+// CTA's barriers.
+template <class View, class Gate>
+__device__ __forceinline__ void copy_units(const View& v, const Cta& x, Ring& r, Unit w, bool is_a,
+                                           Gate gate) {
+  bool shut = true;
+  const uint32_t full0 = map_to_rank(x.full, 0);
+  const int cols = v.cols(), units = v.units();
+  const uint32_t bytes = 2 * (kTileABytes + cols * kDepth);
+  for (int u = x.worker; u < units && r.ok; u += x.workers) {
+    if (u != x.worker) w = locate(v, u, w.p);
+    const Problem& P = v.problem(w.p);
+    int k0, k1;
+    split_range(P, v.parts(w.p), w.split, &k0, &k1);
+    const CUtensorMap* map = is_a ? v.map_a(w.p) : v.map_b(w.p);
+    const int zs = is_a ? v.za(w.p) : v.zb(w.p);
+    const int other = is_a ? P.a_sym : P.b_sym;  // how the transposed blocks come, if any
+    const int mn = is_a ? w.m0 + (int)x.rank * kRows : w.n0 + (int)x.rank * (cols / 2);
+    const int chunks = is_a ? 2 : cols / 128;
+    const int kind0 = is_a ? P.a_kind : P.b_kind;
+    const int diag = other ? mn & ~(kTileRows - 1) : 0;
+    const CUtensorMap* map_t = other ? (is_a ? v.map_a_t(w.p) : v.map_b_t(w.p)) : map;
+    const int kblocks = P.kblocks;
+    int z = w.z * zs, k = k0 * kDepth;
+    if (k0 >= kblocks) {  // the second operand pair of the sum
+      k -= kblocks * kDepth;
+      z += zs > 1;
+    }
+    if (shut) {
+      if (elect_one()) tma_prefetch(k < diag ? map_t : map);
+      __syncwarp();
+      asm volatile("" ::"l"(map), "l"(map_t), "r"(kind0), "r"(mn), "r"(z), "r"(k), "r"(k1),
+                   "r"(kblocks));
+      shut = false;
+      r.ok = gate() && r.ok;
+    }
+    for (int kb = k0; kb < k1 && r.ok; ++kb, k += kDepth) {
+      if (kb == kblocks && kb > k0) {
+        k = 0;
+        z += zs > 1;
+      }
+      if (!__all_sync(0xffffffffu, bar_wait(x.empty + 8 * r.s, r.phase, x.status))) {
+        r.ok = false;
+        break;
+      }
+      if (elect_one()) {
+        const uint32_t bar = full0 + r.s * 8;
+        const uint32_t dst = x.tiles0 + r.s * x.stage_bytes + (is_a ? 0 : kTileABytes);
+        if (is_a && x.rank == 0) bar_expect_tx(x.full + 8 * r.s, bytes);
+        const int kind = k < diag ? other : kind0;
+        const CUtensorMap* m = k < diag ? map_t : map;
+        if (kind == 0) {
+          tma_load(m, dst, bar, k, mn, z);
+        } else if (kind == 2) {
+          tma_load4(m, dst, bar, k, mn >> 6, z);
+        } else {
+          for (int c = 0; c < chunks; ++c)
+            tma_load(m, dst + c * 8192, bar, mn + c * 64, k, z);
+        }
+      }
+      __syncwarp();
+      ++r.count;
+      r.next(x.stages);
+    }
+  }
+  if (shut) r.ok = gate() && r.ok;
+}
+// Leaves no copy in flight: every stage that was filled has been read (its "empty" phase
+// completes), which the waits of a complete run establish here, each of them bounded.
+__device__ __forceinline__ void copy_drain(const Cta& x, Ring& r) {
+  for (int i = 0; i < x.stages && r.ok; ++i) {
+    if (r.count >= (uint32_t)x.stages || r.s < (int)r.count)
+      r.ok = __all_sync(0xffffffffu, bar_wait(x.empty + 8 * r.s, r.phase, x.status));
+    r.next(x.stages);
+  }
+  if (!r.ok)  // a wait ran out: let the copies that were issued land before the CTA ends
+    for (const uint64_t t0 = now_ns(); now_ns() - t0 < 1000000ull;) {}
+}
+
+// Warp 2 of the pair's first CTA: the matrix instructions.
+template <class View>
+__device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, Unit w) {
+  const int cols = v.cols(), units = v.units();
+  for (int u = x.worker; u < units && r.ok; u += x.workers) {
+    if (u != x.worker) w = locate(v, u, w.p);
+    const Problem& P = v.problem(w.p);
+    int k0, k1;
+    split_range(P, v.parts(w.p), w.split, &k0, &k1);
+    if (k0 == k1) continue;  // an empty sum: the epilogue takes zeros
+    // blocks of k's up to these come transposed
+    const int a_diag = P.a_kind ? 0x7fffffff : P.a_sym ? w.m0 / kDepth : 0;
+    const int b_diag = P.b_kind ? 0x7fffffff : P.b_sym ? (w.n0 & ~(kTileRows - 1)) / kDepth : 0;
+    const int buf = r.count & 1;
+    const uint32_t d = x.tmem + buf * (kTmemCols / 2);
+    if (!__all_sync(0xffffffffu,
+                    bar_wait(x.acc_empty + 8 * buf, ((r.count >> 1) & 1) ^ 1, x.status))) {
+      r.ok = false;
+      break;
+    }
+    tc_fence_after();
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!__all_sync(0xffffffffu, bar_wait(x.full + 8 * r.s, r.phase, x.status))) {
+        r.ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool a_mn = kb < a_diag, b_mn = kb < b_diag;
+      const uint32_t idesc = mma_idesc(v.bf16(), a_mn, b_mn, kTileRows, cols);
+      const uint32_t step_a = mma_k_step(a_mn), step_b = mma_k_step(b_mn);
+      if (elect_one()) {
+        const uint32_t addr = x.tiles0 + r.s * x.stage_bytes;
+        uint64_t a = mma_smem_desc(addr, a_mn);
+        uint64_t b = mma_smem_desc(addr + kTileABytes, b_mn);
+#pragma unroll
+        for (int i = 0; i < kDepth / 16; ++i, a += step_a, b += step_b)
+          tc_mma(d, a, b, idesc, kb > k0 || i > 0);
+        tc_commit(x.empty + 8 * r.s);
+        if (kb + 1 == k1) tc_commit(x.acc_full + 8 * buf);
+      }
+      __syncwarp();
+      r.next(x.stages);
+    }
+    ++r.count;
   }
 }
 
-template <int EPI, int DT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    k_product(const __grid_constant__ ProductArgs g) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full =
-      reinterpret_cast<uint64_t*>(smem + kOperandSpace + kEpiWarps * kBlockBytes);
-  uint64_t* empty = full + kMaxStages;
-  uint64_t* acc_full = empty + kMaxStages;
-  uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  volatile uint32_t* last_flag = tmem_slot + 1;
-
+// Warps 4..15: the epilogue. r.count counts tiles. Once a wait has run out, units pass without
+// results, so that the block barriers of the split sums still see every warp.
+template <class View, class Gate>
+__device__ __forceinline__ void finish_units(const View& v, const Cta& x, Ring& r, Unit w,
+                                             Block& b, Gate gate) {
+  bool shut = true;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int worker = blockIdx.x / 2, workers = gridDim.x / 2;
-  const int cols = g.cols, stages = g.stages;
-  const uint32_t stage_bytes = kTileABytes + cols * (kDepth * 2 / 2);
-  const uint32_t tiles0 = smem_addr(smem);
+  const int quad = warp & 3;                 // the tensor-memory lanes this warp can read
+  const int turn = (warp - kFirstEpi) >> 2;  // which of the quadrant's four warps
+  const int cols = v.cols(), units = v.units();
+  for (int u = x.worker; u < units; u += x.workers) {
+    if (u != x.worker) w = locate(v, u, w.p);
+    const Problem& P = v.problem(w.p);
+    int k0, k1;
+    split_range(P, v.parts(w.p), w.split, &k0, &k1);
+    const int buf = r.count & 1;
+    const int64_t row0 = w.m0 + (int)x.rank * kRows + quad * 32;
+    const int N = P.N, n_end = P.n_end, splits = P.splits;
+    const bool sym = P.sym;
+    b.rows = (int)max((int64_t)0, min((int64_t)32, P.M - row0));
+    const typename View::Target target = v.target(w.p, w.z);
+    Sums a;
+    a.tmem = x.tmem + buf * (kTmemCols / 2) + ((uint32_t)(quad * 32) << 16);
+    a.parts = nullptr;
+    a.splits = splits;
+    a.width4 = cols / 4;
+    a.row = quad * 32 + lane;
+    a.done = map_to_rank(x.acc_empty + 8 * buf, 0);
+    // this warp's chunks: accumulator columns turn * 32 + kEpiStep i, of which it takes those inside
+    // the result and not left of a symmetric result's diagonal block
+    auto wanted = [&](int c) {
+      const int col = w.n0 + c;
+      return col < n_end && b.rows > 0 && !(sym && col < w.m0);
+    };
+    a.last = -1;
+    if (splits == 1)
+      for (int c = turn * 32; c < cols; c += kEpiStep)
+        if (wanted(c)) a.last = c;
+    if (shut) {
+      asm volatile("" ::"r"(a.last), "r"(n_end), "r"(splits), "r"(k0), "r"(k1), "r"(b.rows));
+      target.pin();
+      shut = false;
+      r.ok = gate() && r.ok;
+    }
+    if (a.last >= 0) v.prefetch(target, b, row0, w.n0 + turn * 32, n_end);
+    if (k1 > k0 && r.ok) {
+      r.ok =
+          __all_sync(0xffffffffu, bar_wait(x.acc_full + 8 * buf, (r.count >> 1) & 1, x.status));
+      tc_fence_after();
+    }
+    const bool sums = k1 > k0 && r.ok;
+    a.any = sums;
+    bool finished = r.ok;
+    if (splits > 1) {
+      // this CTA's tile of the split: [split][column / 4][row] float4
+      const int64_t tile_id = (int64_t)((u - P.first) / splits) * 2 + x.rank;
+      float4* parts = reinterpret_cast<float4*>(P.split_ws) + tile_id * splits * a.width4 * kRows;
+      float4* mine = parts + (int64_t)w.split * a.width4 * kRows + a.row;
+      for (int c = turn * 32; c < cols; c += kEpiStep) {
+        if (!sums || !wanted(c)) continue;  // a split has at least one k block
+        float f[32];
+        tmem_ld32(a.tmem + c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          __stcg(&mine[(c / 4 + i) * kRows],
+                 make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]));
+      }
+      if (sums) release_sums(a);
+      __threadfence();
+      epilogue_sync();
+      if (threadIdx.x == 32 * kFirstEpi) {
+        const bool all = r.ok && atomicAdd(&P.split_count[tile_id], 1u) == (uint32_t)splits - 1;
+        sts_elem<4>(x.last_flag, all);
+        if (all) P.split_count[tile_id] = 0;  // for the next launch
+      }
+      epilogue_sync();
+      finished = lds_elem<4>(x.last_flag) && r.ok;
+      epilogue_sync();
+      __threadfence();
+      a.parts = parts;
+    } else if (sums && a.last < 0) {
+      release_sums(a);
+    }
+    if (finished) {
+      for (int c = turn * 32; c < cols; c += kEpiStep) {
+        if (!wanted(c)) continue;
+        const int col = w.n0 + c;
+        float f[32];
+        take_sums(a, c, f);
+        v.finish(target, b, f, row0, col, min(32, n_end - col),
+                 N);
+      }
+    }
+    if (sums) ++r.count;
+  }
+  if (shut) r.ok = gate() && r.ok;
+}
 
+constexpr uint32_t kBarrierOffset = (uint32_t)kOperandSpace + kEpiWarps * kBlockBytes;
+
+// Shared set-up of the kernels below: barriers, tensor memory, the pair's first meeting.
+__device__ __forceinline__ void cta_begin(Cta& x, uint8_t* smem, int stages, uint32_t stage_bytes,
+                                          uint32_t* status) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  x.tiles0 = smem_addr(smem);
+  x.full = x.tiles0 + kBarrierOffset;
+  x.empty = x.full + 8 * kMaxStages;
+  x.acc_full = x.empty + 8 * kMaxStages;
+  x.acc_empty = x.acc_full + 16;
+  const uint32_t slot = x.acc_empty + 16;
+  x.last_flag = slot + 4;
+  x.rank = cluster_rank();
+  x.worker = blockIdx.x / 2;
+  x.workers = gridDim.x / 2;
+  x.stages = stages;
+  x.stage_bytes = stage_bytes;
+  x.status = status;
   if (warp == 0) {  // full, empty, acc_full: one arrival; acc_empty: one of each epilogue warp
     constexpr int kBars = 2 * kMaxStages + 4;
-    if (lane < kBars) bar_init(&full[lane], lane < kBars - 2 ? 1 : 2 * kEpiWarps);
+    if (lane < kBars) bar_init(x.full + 8 * lane, lane < kBars - 2 ? 1 : 2 * kEpiWarps);
     bar_init_fence();
   }
-  if (warp == 2) tmem_alloc(tmem_slot, kTmemCols);
-  Unit w = locate(g, worker, 0);  // the first unit is looked up under the set-up's latency
-  if (warp < 2 && elect_one()) tma_prefetch(warp == 0 ? &g.p[w.p].ta : &g.p[w.p].tb);
+  if (warp == 2) tmem_alloc(slot, kTmemCols);
+}
+__device__ __forceinline__ void cta_meet(Cta& x) {
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  x.tmem = lds_elem<4>(x.acc_empty + 16);
+}
+__device__ __forceinline__ void cta_end(const Cta& x) {
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();
   tc_fence_after();
-  const uint32_t tmem = *(volatile uint32_t*)tmem_slot;
-  chain_next();
-  chain_wait();
+  if ((threadIdx.x >> 5) == 2) tmem_free(x.tmem, kTmemCols);
+}
 
-  if (warp < 2) {
-    const bool is_a = warp == 0;
-    const uint32_t full0 = map_to_rank(smem_addr(full), 0);  // the first CTA's barriers count both
-    uint32_t filled = 0;  // stages filled so far
-    int s = 0;
-    uint32_t phase = 1;   // of "empty": the first round finds every stage free
-    bool ok = true;
-    for (int u = worker; u < g.units && ok; u += workers) {
-      if (u != worker) w = locate(g, u, w.p);
-      const Problem& P = g.p[w.p];
-      int k0, k1;
-      split_range(P, w.split, &k0, &k1);
-      const CUtensorMap* map = is_a ? &P.ta : &P.tb;
-      const int kind = is_a ? P.a_mn : P.b_mn, zs = is_a ? P.za : P.zb;
-      const int mn = is_a ? w.m0 + (int)rank * kRows : w.n0 + (int)rank * (cols / 2);
-      const int chunks = is_a ? 2 : cols / 128;
-      const int kblocks = P.kblocks;
-      int z = w.z * zs, k = k0 * kDepth;
-      if (k0 >= kblocks) {  // the second operand pair of the sum
-        k -= kblocks * kDepth;
-        z += zs > 1;
-      }
-      for (int kb = k0; kb < k1; ++kb, k += kDepth) {
-        if (kb == kblocks && kb > k0) {
-          k = 0;
-          z += zs > 1;
-        }
-        if (!__all_sync(0xffffffffu, bar_wait(&empty[s], phase, g.status))) {
-          ok = false;
-          break;
-        }
-        if (elect_one()) {
-          const uint32_t bar = full0 + s * 8;
-          const uint32_t dst = tiles0 + s * stage_bytes + (is_a ? 0 : kTileABytes);
-          if (is_a && rank == 0) bar_expect_tx(&full[s], 2 * stage_bytes);
-          if (kind == 0) {
-            tma_load(map, dst, bar, k, mn, z);
-          } else if (kind == 2) {
-            tma_load4(map, dst, bar, k, mn >> 6, z);
-          } else {
-            for (int c = 0; c < chunks; ++c)
-              tma_load(map, dst + c * 8192, bar, mn + c * 64, k, z);
-          }
-        }
-        __syncwarp();
-        ++filled;
-        if (++s == stages) {
-          s = 0;
-          phase ^= 1;
-        }
-      }
-    }
-    // Leave no copy in flight: every stage that was filled has been read (its "empty" phase
-    // completes), which the waits of a complete run establish here, each of them bounded.
-    for (uint32_t i = 0; i < (uint32_t)stages && ok; ++i) {
-      if (filled >= (uint32_t)stages || s < (int)filled)
-        ok = __all_sync(0xffffffffu, bar_wait(&empty[s], phase, g.status));
-      if (++s == stages) {
-        s = 0;
-        phase ^= 1;
-      }
-    }
-    if (!ok)  // a wait ran out: let the copies that were issued land before the CTA ends
-      for (const uint64_t t0 = now_ns(); now_ns() - t0 < 1000000ull;) {}
-  } else if (warp == 2) {
-    if (rank == 0) {
-      uint32_t tile = 0, phase = 0;
-      int s = 0;
-      bool ok = true;
-      for (int u = worker; u < g.units && ok; u += workers) {
-        if (u != worker) w = locate(g, u, w.p);
-        const Problem& P = g.p[w.p];
-        int k0, k1;
-        split_range(P, w.split, &k0, &k1);
-        if (k0 == k1) continue;  // an empty sum: the epilogue takes zeros
-        const bool a_mn = P.a_mn, b_mn = P.b_mn;
-        const uint32_t idesc = mma_idesc(g.bf16, a_mn, b_mn, kTileRows, cols);
-        const uint32_t step_a = mma_k_step(a_mn), step_b = mma_k_step(b_mn);
-        const int buf = tile & 1;
-        const uint32_t use = tile >> 1;
-        const uint32_t d = tmem + buf * (kTmemCols / 2);
-        if (!__all_sync(0xffffffffu, bar_wait(&acc_empty[buf], (use & 1) ^ 1, g.status))) break;
-        tc_fence_after();
-        for (int kb = k0; kb < k1; ++kb) {
-          if (!__all_sync(0xffffffffu, bar_wait(&full[s], phase, g.status))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t addr = tiles0 + s * stage_bytes;
-            uint64_t a = mma_smem_desc(addr, a_mn);
-            uint64_t b = mma_smem_desc(addr + kTileABytes, b_mn);
-#pragma unroll
-            for (int i = 0; i < kDepth / 16; ++i, a += step_a, b += step_b)
-              tc_mma(d, a, b, idesc, kb > k0 || i > 0);
-            tc_commit(&empty[s]);
-            if (kb + 1 == k1) tc_commit(&acc_full[buf]);
-          }
-          __syncwarp();
-          if (++s == stages) {
-            s = 0;
-            phase ^= 1;
-          }
-        }
-        ++tile;
-      }
-    }
-  } else {
-    const int quad = warp & 3;                    // the tensor-memory lanes this warp can read
-    const int turn = (warp - kFirstEpi) >> 2;     // which of the quadrant's four warps
-    Block b;
-    b.init(tiles0 + (uint32_t)kOperandSpace + (warp - kFirstEpi) * kBlockBytes, lane);
-    uint32_t tile = 0;
-    bool ok = true;  // false once a wait has run out: units pass without results, so that the
-                     // block barriers of the split sums still see every warp
-    for (int u = worker; u < g.units; u += workers) {
-      if (u != worker) w = locate(g, u, w.p);
-      const Problem& P = g.p[w.p];
-      int k0, k1;
-      split_range(P, w.split, &k0, &k1);
-      const int buf = tile & 1;
-      const uint32_t use = tile >> 1;
-      const int64_t row0 = w.m0 + (int)rank * kRows + quad * 32;
-      const int N = P.N, n_end = P.n_end, splits = P.splits;
-      const bool sym = P.sym;
-      b.rows = (int)max((int64_t)0, min((int64_t)32, P.M - row0));
-      Out o;
-      o.out = reinterpret_cast<uint8_t*>(P.out) + w.z * P.out_zs * 2;
-      o.aux = P.aux ? reinterpret_cast<const uint8_t*>(P.aux) + w.z * P.aux_zs * 2 : nullptr;
-      o.bias = P.bias;
-      o.deriv = P.deriv;
-      o.ld = P.ldo;
-      o.ld_aux = P.ld_aux;
-      o.ld_deriv = P.ld_deriv;
-      o.bias_dt = P.bias_dt;
-      o.act = P.act;
-      const Item* item = EPI == EPI_FINAL ? P.items + w.z : nullptr;
-      float alpha = g.alpha;
-      if (g.unit_pow) {
-        const float unit = P.scale[w.z].unit;
-        alpha *= g.unit_pow == 2 ? unit * unit : unit;
-      }
-      Sums a;
-      a.tmem = tmem + buf * (kTmemCols / 2) + ((uint32_t)(quad * 32) << 16);
-      a.parts = nullptr;
-      a.splits = splits;
-      a.width4 = cols / 4;
-      a.row = quad * 32 + lane;
-      a.done = map_to_rank(smem_addr(&acc_empty[buf]), 0);
-      // this warp's chunks: accumulator columns turn * 32 + 128 i, of which it takes those inside
-      // the result and not left of a symmetric result's diagonal block
-      auto wanted = [&](int c) {
-        const int col = w.n0 + c;
-        return col < n_end && b.rows > 0 && !(sym && col < w.m0);
-      };
-      a.last = -1;
-      if (splits == 1)
-        for (int c = turn * 32; c < cols; c += 128)
-          if (wanted(c)) a.last = c;
-      if (k1 > k0 && ok) {
-        ok = __all_sync(0xffffffffu, bar_wait(&acc_full[buf], use & 1, g.status));
-        tc_fence_after();
-      }
-      const bool sums = k1 > k0 && ok;
-      a.any = sums;
-      bool finished = ok;
-      if (splits > 1) {
-        // this CTA's tile of the split: [split][column / 4][row] float4
-        const int64_t tile_id = (int64_t)((u - P.first) / splits) * 2 + rank;
-        float4* parts = reinterpret_cast<float4*>(P.split_ws) + tile_id * splits * a.width4 * kRows;
-        float4* mine = parts + (int64_t)w.split * a.width4 * kRows + a.row;
-        for (int c = turn * 32; c < cols; c += 128) {
-          if (!sums || !wanted(c)) continue;  // a split has at least one k block
-          float v[32];
-          tmem_ld32(a.tmem + c, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            __stcg(&mine[(c / 4 + i) * kRows],
-                   make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
-        }
-        if (sums) release_sums(a);
-        __threadfence();
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
-        if (threadIdx.x == 32 * kFirstEpi) {
-          const bool all = ok && atomicAdd(&P.split_count[tile_id], 1u) == (uint32_t)splits - 1;
-          *last_flag = all;
-          if (all) P.split_count[tile_id] = 0;  // for the next launch
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
-        finished = *last_flag && ok;
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
-        __threadfence();
-        a.parts = parts;
-      } else if (sums && a.last < 0) {
-        release_sums(a);
-      }
-      if (finished) {
-        for (int c = turn * 32; c < cols; c += 128) {
-          if (!wanted(c)) continue;
-          const int col = w.n0 + c;
-          float v[32];
-          take_sums(a, c, v);
-          finish<EPI, DT>(g, o, item, b, v, alpha, row0, col, min(32, n_end - col),
-                          sym && col >= w.m0 + kTileRows, N);
-        }
-      }
-      if (sums) ++tile;
+// ---- the linear layer's products -------------------------------------------------
+struct LinearArgs {
+  CUtensorMap ta, tb;
+  Problem p;
+  Out out;
+  int32_t units, cols, stages, bf16;
+  uint32_t* status;
+};
+
+template <bool EPILOGUE, int DT>  // with bias, activation, residual; or only rounded
+struct LinearView {
+  struct Target {
+    __device__ __forceinline__ void pin() const {}
+  };
+  const LinearArgs& g;
+  __device__ __forceinline__ int count() const { return 1; }
+  __device__ __forceinline__ int units() const { return g.units; }
+  __device__ __forceinline__ int cols() const { return g.cols; }
+  __device__ __forceinline__ bool bf16() const { return DT == DT_BF16; }
+  __device__ __forceinline__ const Problem& problem(int) const { return g.p; }
+  __device__ __forceinline__ const CUtensorMap* map_a(int) const { return &g.ta; }
+  __device__ __forceinline__ const CUtensorMap* map_b(int) const { return &g.tb; }
+  __device__ __forceinline__ const CUtensorMap* map_a_t(int) const { return nullptr; }
+  __device__ __forceinline__ const CUtensorMap* map_b_t(int) const { return nullptr; }
+  __device__ __forceinline__ int za(int) const { return 1; }
+  __device__ __forceinline__ int zb(int) const { return 1; }
+  __device__ __forceinline__ int parts(int) const { return 1; }
+  __device__ __forceinline__ Target target(int, int) const { return Target(); }
+  __device__ __forceinline__ void prefetch(const Target&, const Block&, int64_t, int, int) const {}
+  __device__ __forceinline__ void finish(const Target&, const Block& b, float (&v)[32],
+                                         int64_t row0, int col, int n, int) const {
+    if constexpr (EPILOGUE) {
+      finish_linear<DT>(g.out, b, v, row0, col, n);
+    } else {
+      row_put<DT>(b, v);
+      block_store<2>(b, g.out.out + (row0 * g.out.ld + col) * 2, g.out.ld, n);
     }
   }
-  __syncwarp();
-  tc_fence_before();
-  cluster_sync_all();
-  tc_fence_after();
-  if (warp == 2) tmem_free(tmem, kTmemCols);
+};
+
+template <bool EPILOGUE, int DT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    k_linear(const __grid_constant__ LinearArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const LinearView<EPILOGUE, DT> v{g};
+  const int warp = threadIdx.x >> 5;
+  Cta x;
+  cta_begin(x, smem, g.stages, kTileABytes + g.cols * kDepth, g.status);
+  const Unit w = locate(v, x.worker, 0);  // looked up under the set-up's latency
+  cta_meet(x);
+  chain_next();
+  auto gate = [] {
+    chain_wait();
+    return true;
+  };
+  Ring r;
+  if (warp < 2) {
+    r.phase = 1;  // of "empty": the first round finds every stage free
+    copy_units(v, x, r, w, warp == 0, gate);
+    copy_drain(x, r);
+  } else if (warp == 2) {
+    r.phase = 0;
+    if (x.rank == 0) mma_units(v, x, r, w);
+  } else if (warp >= kFirstEpi) {
+    Block b;
+    b.init(x.tiles0 + (uint32_t)kOperandSpace + (warp - kFirstEpi) * kBlockBytes,
+           threadIdx.x & 31);
+    finish_units(v, x, r, w, b, gate);
+  }
+  cta_end(x);
 }
 
 }  // namespace mx
