@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -48,11 +49,17 @@ constexpr int64_t kMaxDim = 0x7fffff00;  // every dimension (rows, columns) is h
 
 constexpr int kMaxDevices = 64;
 
-int sm_count() {
+int sm_count() {  // of the current device (148 where there is none, as when sizing without a GPU)
+  static std::atomic<int> known[kMaxDevices];
   int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (n <= 0) return 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 // ---- workspace -------------------------------------------------------------
@@ -218,31 +225,49 @@ Shape choose(const std::vector<Product>& ps, int pairs) {
     double time = ps.size() == 1 ? (double)cdiv(units, pairs) * longest
                                  : std::max(longest, work / pairs + 0.5 * longest);
     std::vector<int> splits(ps.size(), 1);
-    if (units * 2 <= pairs) {
-      // so many that each pair gets one split of the longest sums
-      double split_work = 0, split_longest = 0;
-      int64_t tiles = 0, floats = 0, split_units = 0;
-      const double ideal = work / pairs;
-      for (size_t i = 0; i < ps.size(); ++i) {
-        const int64_t kb = blocks_of(ps[i]), t = tiles_of(ps[i], cols) * ps[i].batch;
-        const double c = tile_cycles((double)kb, cols);
-        splits[i] = (int)std::max<int64_t>(
-            1, std::min<int64_t>({kb / 2, (int64_t)(c / std::max(ideal, 1.0)), (int64_t)16}));
-        const double one = tile_cycles((double)cdiv(kb, splits[i]), cols) +
-                           (splits[i] > 1 ? 3000.0 + splits[i] * 2.5 * cols : 0.0);
-        split_units += t * splits[i];
-        split_work += (double)t * splits[i] * one;
-        split_longest = std::max(split_longest, one);
-        if (splits[i] > 1) {
-          tiles += 2 * t;
-          floats += 2 * t * splits[i] * kRows * cols;
+    if (units < pairs) {
+      // a split sum costs its partial tiles' way through memory
+      auto split_cycles = [&](const Product& p, int64_t n) {
+        return tile_cycles((double)cdiv(blocks_of(p), n), cols) +
+               (n > 1 ? 3000.0 + (double)n * 2.5 * cols : 0.0);
+      };
+      std::vector<int> tried(ps.size(), 1);
+      double split_time = 1e300;
+      if (ps.size() == 1) {
+        // the lowest (rounds of units) x (time of one)
+        for (int64_t n = 2; n <= std::min<int64_t>(16, blocks_of(ps[0]) / 2); ++n) {
+          const double t = (double)cdiv(units * n, pairs) * split_cycles(ps[0], n);
+          if (t < split_time) {
+            split_time = t;
+            tried[0] = (int)n;
+          }
         }
+      } else {
+        // so many that each pair gets one split of the longest sums
+        const double ideal = work / pairs;
+        double split_work = 0, split_longest = 0;
+        for (size_t i = 0; i < ps.size(); ++i) {
+          const int64_t kb = blocks_of(ps[i]);
+          const double c = tile_cycles((double)kb, cols);
+          tried[i] = (int)std::max<int64_t>(
+              1, std::min<int64_t>({kb / 2, (int64_t)(c / std::max(ideal, 1.0)), (int64_t)16}));
+          const double one = split_cycles(ps[i], tried[i]);
+          split_work += (double)(tiles_of(ps[i], cols) * ps[i].batch * tried[i]) * one;
+          split_longest = std::max(split_longest, one);
+        }
+        split_time = std::max(split_longest, split_work / pairs);
       }
-      const double split_time = ps.size() == 1
-                                    ? (double)cdiv(split_units, pairs) * split_longest
-                                    : std::max(split_longest, split_work / pairs);
-      if (split_time < time && tiles <= kSplitTiles && floats <= kSplitFloats) time = split_time;
-      else splits.assign(ps.size(), 1);
+      int64_t tiles = 0, floats = 0;
+      for (size_t i = 0; i < ps.size(); ++i)
+        if (tried[i] > 1) {
+          const int64_t t = 2 * tiles_of(ps[i], cols) * ps[i].batch;
+          tiles += t;
+          floats += t * tried[i] * kRows * cols;
+        }
+      if (split_time < time && tiles <= kSplitTiles && floats <= kSplitFloats) {
+        time = split_time;
+        splits = tried;
+      }
     }
     if (time < best_time) {
       best_time = time;
@@ -832,7 +857,7 @@ ta_status check_space(const Arena& need, void* ws, size_t bytes, const uint32_t*
   return TA_OK;
 }
 
-// A few rows of A against all of B: up to 8, read where they lie.
+// A few rows of A against all of B, read where they lie.
 bool few_rows(const Product& p) {
   if (p.M < 1 || p.M > kFewMax || p.a.k < 1) return false;
   if (p.a.mn_major && p.M > 1) return false;
@@ -883,8 +908,7 @@ ta_status run_few(const Product& p, const Out& out, float* part, int64_t room,
   const bool cols = p.b.mn_major;
   if (g.tokens == 1) return launch_few<DT, 1>(g, cols, room, stream);
   if (g.tokens == 2) return launch_few<DT, 2>(g, cols, room, stream);
-  if (g.tokens <= 4) return launch_few<DT, 4>(g, cols, room, stream);
-  return launch_few<DT, 8>(g, cols, room, stream);
+  return launch_few<DT, kFewMax>(g, cols, room, stream);
 }
 
 // The products of one linear call: counters are cleared where a launch may split its sums.
@@ -902,7 +926,7 @@ struct GradLines {
   Lines dz_t, dz_o, x, w;  // dz as tokens x fan_out and as fan_out x tokens; x, w over k
   bool dw_io = false;      // dw's rows are fan_in
   bool make_dz = false;
-  int64_t row_parts = 0, ld_dz = 0;
+  int64_t row_parts = 0, col_blocks = 0, col_threads = 0, ld_dz = 0;
 };
 
 ta_status prepare_grad(const ta_linear_grad* op, GradLines* g) {
@@ -933,11 +957,15 @@ ta_status prepare_grad(const ta_linear_grad* op, GradLines* g) {
   const int64_t stride = op->tokens > 1 ? op->dy_stride : up8(op->fan_out);
   g->make_dz = op->deriv_dev || !aligned16(op->dy_dev) || stride % 8;
   g->ld_dz = g->make_dz ? up8(op->fan_out) : stride;
-  // rows are split until the blocks of 256 columns fill the SMs some four times
-  if (op->db_dev || g->make_dz)
+  // rows are split until there are some eight blocks for every SM, of 8 rows or more
+  if (op->db_dev || g->make_dz) {
+    const int64_t pieces = std::max<int64_t>(1, cdiv(op->fan_out, 8));
+    g->col_blocks = cdiv(pieces, kEltThreads);
+    g->col_threads = cdiv(cdiv(pieces, g->col_blocks), 32) * 32;
     g->row_parts = std::max<int64_t>(
-        1, std::min<int64_t>(cdiv(op->tokens, 16),
-                             cdiv(4 * sm_count(), std::max<int64_t>(1, cdiv(op->fan_out, 256)))));
+        1, std::min<int64_t>({cdiv(op->tokens, 8), cdiv(8 * sm_count(), g->col_blocks),
+                              (int64_t)256}));
+  }
   return TA_OK;
 }
 
@@ -1085,12 +1113,12 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
     const bool bf16 = op->dtype == TA_BF16;
     const void* dz = g.make_dz ? (const void*)s.dz : op->dy_dev;
     if (O > 0 && (g.make_dz || op->db_dev)) {
-      const dim3 grid((unsigned)cdiv(O, 256), (unsigned)g.row_parts);
-      MX_OK(launch(k_dz, grid, kEltThreads, 0, stream, op->dy_dev, op->dy_stride, op->deriv_dev,
+      const dim3 grid((unsigned)g.col_blocks, (unsigned)g.row_parts);
+      MX_OK(launch(k_dz, grid, (int)g.col_threads, 0, stream, op->dy_dev, op->dy_stride, op->deriv_dev,
                    (int)up8(O), (int)T, (int)O, (int)op->dtype, g.make_dz ? s.dz : nullptr,
                    (int)g.ld_dz, op->db_dev ? s.part : nullptr));
       if (op->db_dev)
-        MX_OK(launch(k_bias_grad, dim3((unsigned)cdiv(O, kEltThreads)), kEltThreads, 0, stream,
+        MX_OK(launch(k_bias_grad, dim3((unsigned)cdiv(O, 32)), kEltThreads, 0, stream,
                      s.part, (int)g.row_parts, (int)O, op->db_dev, (int)op->bias_dtype));
     }
     auto result = [](void* p, int64_t ld) {

@@ -3,8 +3,9 @@
 //
 // A tile of the product engine has 256 rows; with one token its matrix instructions would work
 // on zeros, and its copies, one stage at a time and CTA pair, reach some 2.6 TB/s (45 us at
-// 4096 > 14336). Here every lane has several 16-byte loads of B under way, which is what HBM
-// asks for. Two forms, by which dimension of B is contiguous:
+// 4096 > 14336, bf16, for 1 to 16 tokens). Here every lane has several 16-byte loads of B under
+// way, which is what HBM asks for: 23 us for one token (5.1 TB/s), 34 us for two, 48 us for four,
+// where a lane's arithmetic takes over; beyond, the tiles are faster. Two forms, by which dimension of B is contiguous:
 //   k_few_rows: the sum's (an output by input weight): a warp takes four rows of B;
 //   k_few_cols: the result's: a lane takes eight columns, the sum is split over the warps of a
 //               block and over blocks, and k_few_finish adds the blocks' parts in order.
@@ -15,7 +16,7 @@
 namespace ta {
 namespace mx {
 
-constexpr int kFewMax = 8;   // rows of A
+constexpr int kFewMax = 4;   // rows of A
 constexpr int kFewRows = 4;  // rows of B a warp takes
 
 struct FewArgs {
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(256) k_few_cols(const __grid_constant__ FewArg
   const int k0 = (int)((int64_t)g.K * blockIdx.y / gridDim.y);
   const int k1 = (int)((int64_t)g.K * (blockIdx.y + 1) / gridDim.y);
   // a stretch of A in shared memory, a step's tokens side by side
-  constexpr int kStretch = 256;
+  constexpr int kStretch = 1024 / T;
   __shared__ __align__(16) float xs[kStretch][T];
   float acc[T][8] = {};
   for (int kc = k0; kc < k1; kc += kStretch) {

@@ -226,8 +226,9 @@ class _LinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():  # create_graph=True
+            raise NotImplementedError("linear_act is differentiable once")
         nx, nw, nb, nr, _ = ctx.needs_input_grad
         dx = dw = db = None
         if nx or nw or nb:
