@@ -408,16 +408,31 @@ ta_status run_linear(const Product& p, const Out& out, float* split_ws, uint32_t
 // (The product of two polynomials is at most the square of one, P A a few times A.)
 constexpr float kScaleX = 1024.f, kScaleA = 1024.f, kScaleP = 256.f, kScaleT = 512.f;
 
+// Two steps can go as a pair. With A the Gram matrix of X, P and P' the polynomials of the steps,
+//   T = P A,  A' = P T  (the Gram matrix of P X, without forming P X),  Q = P' P,  X <- Q X:
+// in units of a side^3 product and with r = long / short side, 3 r + 5 for two steps against
+// 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the unrounded input,
+// so X is never rounded while its small singular values still drown in the error of the large
+// ones: that halves the error (2-norm, on spectra that fall by 50 within a quarter of their
+// length over a floor: 1.3e-3 against 2.0e-3; bf16 operands would leave 2e-2). A later pair
+// saves products only where r is well over 1, and rounds P and A' where X was rounded before: its
+// error falls with the side (2.8e-3, 2.2e-3 in all at sides of 512 and 1024, 1.4e-3 in the
+// tests' largest). So the later steps go in pairs ("deep") from a side of 2048 and r of 2 on
+// (14336 x 4096: 2.25 ms against 2.6), and one by one elsewhere. Three steps at once would lose
+// 1e-2.
+bool deep_pairs(int64_t side, int64_t length) { return side >= 2048 && length >= 2 * side; }
+
 struct Class {  // matrices of one shape
   int64_t rows = 0, cols = 0, ld = 0, side = 0, lds = 0, count = 0;
   int first = 0;  // first table slot
-  bool pair = false, tall = false;
+  bool pair = false, tall = false, deep = false;
   __half *x0 = nullptr, *x1 = nullptr, *square[3] = {nullptr, nullptr, nullptr};
   int64_t xs() const { return rows * ld; }
   int64_t ss() const { return side * lds; }
 };
 
 struct OrthoPlan {
+  std::vector<int> chains;  // first class of each chain
   std::vector<Class> classes;
   std::vector<std::vector<int>> members;  // tensors of each class
   int64_t items = 0;
@@ -464,6 +479,7 @@ ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_option
       c.ld = up32(t.cols);  // whole epilogue chunks
       c.tall = t.rows > t.cols;
       c.side = std::min(t.rows, t.cols);
+      c.deep = deep_pairs(c.side, std::max(t.rows, t.cols));
       c.lds = up32(c.side);
       c.pair = pair;
       plan->classes.push_back(c);
@@ -472,6 +488,22 @@ ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_option
     plan->classes[it->second].count += t.batch;
     plan->members[it->second].push_back(i);
   }
+  // chains: up to kMaxClasses classes of one sequence of phases each
+  OrthoPlan sorted;
+  for (int deep = 0; deep < 2; ++deep) {
+    int in_chain = kMaxClasses;
+    for (size_t i = 0; i < plan->classes.size(); ++i) {
+      if (plan->classes[i].deep != (deep == 1)) continue;
+      if (in_chain == kMaxClasses) {
+        sorted.chains.push_back((int)sorted.classes.size());
+        in_chain = 0;
+      }
+      ++in_chain;
+      sorted.classes.push_back(plan->classes[i]);
+      sorted.members.push_back(plan->members[i]);
+    }
+  }
+  *plan = sorted;
   for (Class& c : plan->classes) {
     c.first = (int)plan->items;
     plan->items += c.count;
@@ -491,7 +523,7 @@ struct OrthoSpace {
   float* split_ws;
 };
 
-int chains_of(const OrthoPlan& plan) { return (int)cdiv((int64_t)plan.classes.size(), kMaxClasses); }
+int chains_of(const OrthoPlan& plan) { return (int)plan.chains.size(); }
 
 OrthoSpace carve_ortho(OrthoPlan* plan, Arena* a) {
   OrthoSpace s;
@@ -510,15 +542,7 @@ OrthoSpace carve_ortho(OrthoPlan* plan, Arena* a) {
   return s;
 }
 
-// Steps go in pairs. With A the Gram matrix of X, P and P' the polynomials of two steps,
-//   T = P A,  A' = P T  (the Gram matrix of P X, without forming P X),  Q = P' P,  X <- Q X:
-// in units of a side^3 product and with r = long / short side, 3 r + 5 for two steps against
-// 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the unrounded
-// input. Rounding A, and not X, costs accuracy where A's small eigenvalues drown in the error
-// of its large ones; over two steps (with the input exact) they do not: 1.3e-3 to 1.7e-3 of the
-// result on spectra that decay by 50 to 800, against 1.8e-3 to 2.6e-3 one by one (bf16
-// operands: 2e-2). Over three they would (1e-2).
-int chain_phases(const ta_ortho_options* o, Phase* out) {
+int chain_phases(const ta_ortho_options* o, bool deep, Phase* out) {
   int n = 0;
   auto add = [&](int type, int end, int a, int b, int to, float alpha) -> Phase& {
     Phase& p = out[n++];
@@ -541,7 +565,7 @@ int chain_phases(const ta_ortho_options* o, Phase* out) {
     p.aux = (int8_t)gram;
   };
   for (int step = 0; step < o->steps;) {
-    const bool first = step == 0, two = step + 1 < o->steps;
+    const bool first = step == 0, two = step + 1 < o->steps && (first || deep);
     add(PH_GRAM, END_SCALE, x, x, gram, first ? kScaleA : kScaleA / (kScaleX * kScaleX))
         .unit_pow = first ? 2 : 0;
     polynomial(step);
@@ -575,7 +599,7 @@ ta_status run_chain(const std::vector<Class>& classes, const ta_ortho_options* o
   static thread_local ChainArgs g;  // some 20 KB
   memset(&g, 0, sizeof(g));
   g.classes = (int32_t)classes.size();
-  g.phases = chain_phases(o, g.phase);
+  g.phases = chain_phases(o, classes[0].deep, g.phase);
 
   auto square = [](const Class& c, int i, bool transposed = false) {
     Operand q;
@@ -748,9 +772,9 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
                o->nesterov, o->eps));
 
   for (int i = 0; i < chains_of(plan); ++i) {
-    const size_t lo = (size_t)i * kMaxClasses;
-    const std::vector<Class> part(plan.classes.begin() + lo,
-                                  plan.classes.begin() + std::min(plan.classes.size(), lo + kMaxClasses));
+    const std::vector<Class> part(
+        plan.classes.begin() + plan.chains[i],
+        i + 1 < chains_of(plan) ? plan.classes.begin() + plan.chains[i + 1] : plan.classes.end());
     MX_OK(run_chain(part, o, sp, sp.chain + 2 * i, status, stream));
   }
   return TA_OK;
