@@ -720,3 +720,47 @@ def test_muon_non_finite_gradient_stays_in_its_matrix():
     Muon(ps).step()
     assert torch.isnan(ps[1]).all()
     assert torch.isfinite(ps[0]).all() and torch.isfinite(ps[2]).all()
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(2048, 4200), (4100, 2050)])
+def test_ortho_steps_in_pairs(shape):
+    """Sides from which the later steps also go in pairs."""
+    from turboadam_b200 import orthogonalize
+
+    for dtype in (torch.bfloat16, torch.float32):
+        x = grad_like(*shape, dtype=dtype)
+        assert rel(orthogonalize(x, dtype=torch.float32), ortho64(x)) <= ORTHO_TOL
+
+
+def test_ortho_split_sums_and_mixed_lists():
+    """A long sum over few tiles (split over SMs), beside shapes of both sequences of steps and
+    both kinds of result, in one call of the optimizer."""
+    from turboadam_b200 import Muon
+
+    shapes = [(40, 9000), (9000, 24), (2048, 4100), (130, 130), (40, 9000)]
+    for dtype in (torch.float32, torch.bfloat16):
+        ps = [torch.nn.Parameter(torch.zeros(s, device="cuda", dtype=dtype)) for s in shapes]
+        opt = Muon(ps, lr=1.0, weight_decay=0.0, momentum=0.0, nesterov=False)
+        for i, p in enumerate(ps):
+            p.grad = grad_like(*p.shape, seed=i).to(dtype)
+        opt.step()
+        for p in ps:
+            want = ortho64(p.grad) * math.sqrt(max(1.0, p.shape[0] / p.shape[1]))
+            tol = ORTHO_TOL + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+            assert rel(-p.detach(), want) <= tol
+
+
+def test_residual_mlp_example_learns():
+    """The layers, the orthogonal start and both optimizers together: the loss falls by far."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "train_residual_mlp.py")
+    spec = importlib.util.spec_from_file_location("train_residual_mlp", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses = example.train(steps=120, width=128, depth=2, batch=256)
+    assert all(math.isfinite(v) for v in losses)
+    assert sum(losses[-10:]) < 0.2 * sum(losses[:10])
