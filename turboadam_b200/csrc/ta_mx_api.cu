@@ -436,11 +436,16 @@ struct OrthoPlan {
   std::vector<Class> classes;
   std::vector<std::vector<int>> members;  // tensors of each class
   int64_t items = 0;
+  int64_t elems = 0;
   int64_t chunks = 0;
 };
 
-int64_t chunk_elems(int64_t n) {
-  return std::max<int64_t>(4096, cdiv(cdiv(n, kMaxChunks), 2048) * 2048);
+// Elements of a block of the elementwise passes: some four blocks for every SM over the whole list
+// (a block's lookups and sums cost a few microseconds, its loads hide each other), at most
+// kMaxChunks of a matrix.
+int64_t chunk_elems(int64_t n, int64_t total) {
+  const int64_t share = cdiv(total, 4 * sm_count()), least = cdiv(n, kMaxChunks);
+  return cdiv(std::max<int64_t>({4096, share, least}), 2048) * 2048;
 }
 
 ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_options* o,
@@ -504,10 +509,11 @@ ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_option
     }
   }
   *plan = sorted;
+  for (const Class& c : plan->classes) plan->elems += c.count * c.rows * c.cols;
   for (Class& c : plan->classes) {
     c.first = (int)plan->items;
     plan->items += c.count;
-    plan->chunks += c.count * cdiv(c.rows * c.cols, chunk_elems(c.rows * c.cols));
+    plan->chunks += c.count * cdiv(c.rows * c.cols, chunk_elems(c.rows * c.cols, plan->elems));
     if (plan->items > 0x7fffffff || plan->chunks > 0x7fffffff)
       return ta_fail(TA_ERR_UNSUPPORTED, "too many matrices in one call");
   }
@@ -717,7 +723,7 @@ ta_status run_ortho(const ta_ortho_tensor* ts, const ta_ortho_options* o, OrthoP
   int64_t chunk = 0;
   for (size_t k = 0; k < plan.classes.size(); ++k) {
     const Class& c = plan.classes[k];
-    const int64_t n = c.rows * c.cols, ce = chunk_elems(n), stored = c.xs() * (c.pair ? 2 : 1);
+    const int64_t n = c.rows * c.cols, ce = chunk_elems(n, plan.elems), stored = c.xs() * (c.pair ? 2 : 1);
     int64_t slot = c.first;
     for (int i : plan.members[k]) {
       const ta_ortho_tensor& t = ts[i];
