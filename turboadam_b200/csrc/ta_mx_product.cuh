@@ -14,12 +14,14 @@
 // give every pair of SMs a share of a small result. Two accumulators let a tile's epilogue run
 // under the next tile's products.
 //
-// Roles of the 16 warps: warps 0 and 1 issue the TMA loads of A and of B, warp 2
-// (of the pair's first CTA) the matrix instructions, warp 3 rests, warps 4..15
-// are the epilogue, three to each 32-row quadrant of tensor memory. They take the
+// Roles of the 12 warps: warps 0 and 1 issue the TMA loads of A and of B, warp 2
+// (of the pair's first CTA) the matrix instructions, warp 3 rests, warps 4..11
+// are the epilogue, two to each 32-row quadrant of tensor memory. They take the
 // tile's 32-column chunks in turn and pass them through shared memory, so that
-// every global access covers whole sectors of consecutive lines. Twelve warps
-// leave each thread 128 registers; sixteen left 96, and spilled.
+// every global access covers whole sectors of consecutive lines. Eight warps
+// leave each thread 168 registers; twelve and sixteen spilled and were slower
+// (12 x 768 x 768 orthogonalised: 207, 244 and 255 us), four had too little
+// under way (225 us).
 //
 // Long sums with few tiles (the Gram matrix of a wide matrix; few tokens) are
 // split over k: each split leaves its fp32 tile in the workspace, and the last
@@ -631,7 +633,7 @@ __device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, 
   }
 }
 
-// Warps 4..15: the epilogue. r.count counts tiles. Once a wait has run out, units pass without
+// Warps 4..11: the epilogue. r.count counts tiles. Once a wait has run out, units pass without
 // results, so that the block barriers of the split sums still see every warp.
 template <class View, class Gate>
 __device__ __forceinline__ void finish_units(const View& v, const Cta& x, Ring& r, Unit w,
@@ -639,7 +641,7 @@ __device__ __forceinline__ void finish_units(const View& v, const Cta& x, Ring& 
   bool shut = true;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = warp & 3;                 // the tensor-memory lanes this warp can read
-  const int turn = (warp - kFirstEpi) >> 2;  // which of the quadrant's four warps
+  const int turn = (warp - kFirstEpi) >> 2;  // which of the quadrant's warps
   const int cols = v.cols(), units = v.units();
   for (int u = x.worker; u < units; u += x.workers) {
     if (u != x.worker) w = locate(v, u, w.p);
