@@ -764,3 +764,25 @@ def test_residual_mlp_example_learns():
     losses = example.train(steps=120, width=128, depth=2, batch=256)
     assert all(math.isfinite(v) for v in losses)
     assert sum(losses[-10:]) < 0.2 * sum(losses[:10])
+
+
+def test_operators_on_two_streams_at_once():
+    """Independent calls on two streams: each chain's blocks are resident together whatever else
+    runs, and workspaces are not shared."""
+    from turboadam_b200 import linear_act, orthogonalize
+
+    xs = [torch.randn(12, 256, 320, device="cuda"), torch.randn(40, 100, 90, device="cuda")]
+    w = torch.randn(512, 320, device="cuda").bfloat16()
+    t = torch.randn(900, 320, device="cuda").bfloat16()
+    want = [orthogonalize(x) for x in xs] + [linear_act(t, w, activation="silu")]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((orthogonalize(xs[i]), linear_act(t, w, activation="silu")))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, y in got[i]:
+            assert torch.equal(o, want[i]) and torch.equal(y, want[2])

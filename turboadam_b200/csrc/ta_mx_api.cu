@@ -370,27 +370,30 @@ int stages_of(int cols) {
                                kOperandSpace / (size_t)(kTileABytes + cols * kDepth));
 }
 
-// One linear product. split_ws / split_count: kSplitFloats and kSplitTiles of them.
+// One product with its epilogue, or up to two plain ones, in one launch. split_ws / split_count:
+// kSplitFloats and kSplitTiles of them.
 template <bool EPILOGUE, int DT>
-ta_status run_linear(const Product& p, const Out& out, float* split_ws, uint32_t* split_count,
-                     uint32_t* status, cudaStream_t stream) {
+ta_status run_linear(const std::vector<Product>& ps, const std::vector<Out>& outs, float* split_ws,
+                     uint32_t* split_count, uint32_t* status, cudaStream_t stream) {
   static int found[kMaxDevices];
   int pairs = 0;
   MX_OK(bind_device());
   MX_OK(pairs_of(k_linear<EPILOGUE, DT>, found, &pairs));
-  const std::vector<Product> ps(1, p);
   const Shape shape = choose(ps, pairs);
   LinearArgs g;
   memset(&g, 0, sizeof(g));
   int64_t split_tiles = 0;
-  const int64_t units = place_products(ps, shape, split_ws, split_count, &g.p, &split_tiles);
+  const int64_t units = place_products(ps, shape, split_ws, split_count, g.p, &split_tiles);
   if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
   if (units == 0) return TA_OK;
-  if (p.a.k > 0) {
-    MX_OK(make_map(&g.ta, p.a, DT == DT_BF16, kRows));
-    MX_OK(make_map(&g.tb, p.b, DT == DT_BF16, shape.cols / 2));
+  for (size_t i = 0; i < ps.size(); ++i) {
+    if (ps[i].a.k > 0) {
+      MX_OK(make_map(&g.maps[i][0], ps[i].a, DT == DT_BF16, kRows));
+      MX_OK(make_map(&g.maps[i][1], ps[i].b, DT == DT_BF16, shape.cols / 2));
+    }
+    g.out[i] = outs[i];
   }
-  g.out = out;
+  g.count = (int32_t)ps.size();
   g.units = (int32_t)units;
   g.cols = shape.cols;
   g.stages = stages_of(shape.cols);
@@ -814,25 +817,39 @@ bool lines_of(const void* p, int64_t mn, int64_t k, int64_t s_mn, int64_t s_k, L
   return l->lines <= 1 || l->stride >= l->len;
 }
 
-ta_status operand_of(const void* p, int64_t mn, int64_t k, const Lines& l, uint16_t* copy,
-                     Operand* o, cudaStream_t stream) {
-  o->mn = mn;
-  o->k = k;
-  o->mn_major = l.mn_major;
-  o->z = 1;
+// The operand, and the copy it needs first (job->rows > 0).
+Operand operand_of(const void* p, int64_t mn, int64_t k, const Lines& l, uint16_t* copy,
+                   CopyJob* job) {
+  Operand o;
+  o.mn = mn;
+  o.k = k;
+  o.mn_major = l.mn_major;
+  o.z = 1;
   if (l.direct) {
-    o->p = p;
-    o->ld = l.stride;
+    o.p = p;
+    o.ld = l.stride;
   } else {
-    o->p = copy;
-    o->ld = up8(l.len);
-    const dim3 grid((unsigned)std::min<int64_t>(cdiv(l.len, kEltThreads), 64),
-                    (unsigned)std::min<int64_t>(l.lines, 4096));
-    MX_OK(launch(k_copy_rows, grid, kEltThreads, 0, stream, reinterpret_cast<const uint16_t*>(p),
-                 l.stride, (int)l.lines, (int)l.len, copy, (int)o->ld));
+    o.p = copy;
+    o.ld = up8(l.len);
+    job->src = reinterpret_cast<const uint16_t*>(p);
+    job->stride = l.stride;
+    job->dst = copy;
+    job->rows = (int32_t)l.lines;
+    job->cols = (int32_t)l.len;
+    job->ld = (int32_t)o.ld;
   }
-  o->zs = o->ld * l.lines;
-  return TA_OK;
+  o.zs = o.ld * l.lines;
+  return o;
+}
+
+ta_status run_copies(CopyArgs a, cudaStream_t stream) {
+  if (a.job[0].rows == 0) std::swap(a.job[0], a.job[1]);
+  if (a.job[0].rows == 0) return TA_OK;
+  const int64_t cols = std::max(a.job[0].cols, a.job[1].cols),
+                rows = std::max(a.job[0].rows, a.job[1].rows);
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(cols, kEltThreads), 64),
+                  (unsigned)std::min<int64_t>(rows, 4096), a.job[1].rows ? 2 : 1);
+  return launch(k_copy_rows, grid, kEltThreads, 0, stream, a);
 }
 
 size_t copy_elems(const Lines& l) { return l.direct ? 0 : (size_t)(up8(l.len) * l.lines); }
@@ -941,13 +958,22 @@ ta_status run_few(const Product& p, const Out& out, float* part, int64_t room,
   return launch_few<DT, kFewMax>(g, cols, room, stream);
 }
 
-// The products of one linear call: counters are cleared where a launch may split its sums.
-ta_status plain_product(const Product& p, const Out& out, bool bf16, const LinearSpace& s,
-                        uint32_t* status, cudaStream_t stream, bool epilogue) {
-  if (few_rows(p) && p.M * p.N <= kSplitFloats)
-    return bf16 ? run_few<DT_BF16>(p, out, s.split_ws, kSplitFloats, stream)
-                : run_few<DT_F16>(p, out, s.split_ws, kSplitFloats, stream);
-  auto run = [&](auto fn) { return fn(p, out, s.split_ws, s.split_count, status, stream); };
+// The products of one linear call.
+ta_status run_products(std::vector<Product> ps, std::vector<Out> outs, bool bf16,
+                       const LinearSpace& s, uint32_t* status, cudaStream_t stream,
+                       bool epilogue) {
+  for (size_t i = 0; i < ps.size();) {
+    if (few_rows(ps[i]) && ps[i].M * ps[i].N <= kSplitFloats) {
+      MX_OK(bf16 ? run_few<DT_BF16>(ps[i], outs[i], s.split_ws, kSplitFloats, stream)
+                 : run_few<DT_F16>(ps[i], outs[i], s.split_ws, kSplitFloats, stream));
+      ps.erase(ps.begin() + i);
+      outs.erase(outs.begin() + i);
+    } else {
+      ++i;
+    }
+  }
+  if (ps.empty()) return TA_OK;
+  auto run = [&](auto fn) { return fn(ps, outs, s.split_ws, s.split_count, status, stream); };
   if (epilogue) return bf16 ? run(run_linear<true, DT_BF16>) : run(run_linear<true, DT_F16>);
   return bf16 ? run(run_linear<false, DT_BF16>) : run(run_linear<false, DT_F16>);
 }
@@ -1089,8 +1115,11 @@ ta_status ta_linear_forward(const ta_linear* op, void* workspace_dev, size_t wor
     cudaStream_t stream = (cudaStream_t)stream_;
     Product p;
     if (op->fan_in > 0) {
-      MX_OK(operand_of(op->x_dev, op->tokens, op->fan_in, x, s.xc, &p.a, stream));
-      MX_OK(operand_of(op->w_dev, op->fan_out, op->fan_in, w, s.wc, &p.b, stream));
+      CopyArgs copies;
+      memset(&copies, 0, sizeof(copies));
+      p.a = operand_of(op->x_dev, op->tokens, op->fan_in, x, s.xc, &copies.job[0]);
+      p.b = operand_of(op->w_dev, op->fan_out, op->fan_in, w, s.wc, &copies.job[1]);
+      MX_OK(run_copies(copies, stream));
     }
     p.M = op->tokens;
     p.N = op->fan_out;
@@ -1105,7 +1134,7 @@ ta_status ta_linear_forward(const ta_linear* op, void* workspace_dev, size_t wor
     out.act = op->activation;
     out.deriv = op->deriv_dev;
     out.ld_deriv = up8(op->fan_out);
-    return plain_product(p, out, op->dtype == TA_BF16, s, status_dev, stream, true);
+    return run_products({p}, {out}, op->dtype == TA_BF16, s, status_dev, stream, true);
   } catch (const std::exception& e) {
     return ta_fail(TA_ERR_INVALID, e.what());
   }
@@ -1168,21 +1197,27 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
       o.zs = g.ld_dz * T;
       return o;
     };
+    // both products in one launch: each fills the other's last round of tiles
+    std::vector<Product> ps;
+    std::vector<Out> outs;
+    CopyArgs copies;
+    memset(&copies, 0, sizeof(copies));
     if (op->dx_dev && T > 0 && I > 0) {
       Product p;
       if (O > 0) {
         p.a = dz_operand(false);
-        MX_OK(operand_of(op->w_dev, I, O, g.w, s.lin.wc, &p.b, stream));
+        p.b = operand_of(op->w_dev, I, O, g.w, s.lin.wc, &copies.job[0]);
       }
       p.M = T;
       p.N = I;
-      MX_OK(plain_product(p, result(op->dx_dev, I), bf16, s.lin, status_dev, stream, false));
+      ps.push_back(p);
+      outs.push_back(result(op->dx_dev, I));
     }
     if (op->dw_dev && O > 0 && I > 0) {
       Product p;
       Operand xo, zo;
       if (T > 0) {
-        MX_OK(operand_of(op->x_dev, I, T, g.x, s.lin.xc, &xo, stream));
+        xo = operand_of(op->x_dev, I, T, g.x, s.lin.xc, &copies.job[1]);
         zo = dz_operand(true);
       }
       p.a = g.dw_io ? xo : zo;
@@ -1190,9 +1225,11 @@ ta_status ta_linear_backward(const ta_linear_grad* op, void* workspace_dev,
       p.M = g.dw_io ? I : O;
       p.N = g.dw_io ? O : I;
       const int64_t ldo = op->dw_strides[g.dw_io ? 1 : 0];
-      MX_OK(plain_product(p, result(op->dw_dev, p.M > 1 ? ldo : p.N), bf16, s.lin, status_dev,
-                          stream, false));
+      ps.push_back(p);
+      outs.push_back(result(op->dw_dev, p.M > 1 ? ldo : p.N));
     }
+    MX_OK(run_copies(copies, stream));
+    if (!ps.empty()) MX_OK(run_products(ps, outs, bf16, s.lin, status_dev, stream, false));
     return TA_OK;
   } catch (const std::exception& e) {
     return ta_fail(TA_ERR_INVALID, e.what());

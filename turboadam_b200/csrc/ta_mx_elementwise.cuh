@@ -279,14 +279,24 @@ __global__ void __launch_bounds__(kEltThreads)
 }
 
 // ---- operand copies --------------------------------------------------------------
-// rows x cols 16-bit elements into rows of ld elements (TMA reads rows that start on 16 bytes).
-__global__ void __launch_bounds__(kEltThreads)
-    k_copy_rows(const uint16_t* src, int64_t stride, int rows, int cols, uint16_t* dst, int ld) {
+// rows x cols 16-bit elements into rows of ld elements (TMA reads rows that start on 16 bytes); up
+// to two matrices, one for each z of the grid.
+struct CopyJob {
+  const uint16_t* src;
+  int64_t stride;
+  uint16_t* dst;
+  int32_t rows, cols, ld;
+};
+struct CopyArgs {
+  CopyJob job[2];
+};
+__global__ void __launch_bounds__(kEltThreads) k_copy_rows(const __grid_constant__ CopyArgs a) {
   chain_next();
   chain_wait();
-  for (int r = blockIdx.y; r < rows; r += gridDim.y)
-    for (int c = blockIdx.x * kEltThreads + threadIdx.x; c < cols; c += gridDim.x * kEltThreads)
-      dst[(int64_t)r * ld + c] = src[(int64_t)r * stride + c];
+  const CopyJob& j = a.job[blockIdx.z];
+  for (int r = blockIdx.y; r < j.rows; r += gridDim.y)
+    for (int c = blockIdx.x * kEltThreads + threadIdx.x; c < j.cols; c += gridDim.x * kEltThreads)
+      j.dst[(int64_t)r * j.ld + c] = j.src[(int64_t)r * j.stride + c];
 }
 
 // ---- gradient of the activation, and of the bias -----------------------------------

@@ -772,41 +772,45 @@ __device__ __forceinline__ void cta_end(const Cta& x) {
 }
 
 // ---- the linear layer's products -------------------------------------------------
+constexpr int kLinearProducts = 2;  // a layer's two gradients go in one launch
 struct LinearArgs {
-  CUtensorMap ta, tb;
-  Problem p;
-  Out out;
-  int32_t units, cols, stages, bf16;
+  CUtensorMap maps[kLinearProducts][2];
+  Problem p[kLinearProducts];
+  Out out[kLinearProducts];
+  int32_t count, units, cols, stages;
   uint32_t* status;
 };
 
-template <bool EPILOGUE, int DT>  // with bias, activation, residual; or only rounded
+template <bool EPILOGUE, int DT>  // with bias, activation, residual (one product); or only rounded
 struct LinearView {
   struct Target {
+    int p;
     __device__ __forceinline__ void pin() const {}
   };
   const LinearArgs& g;
-  __device__ __forceinline__ int count() const { return 1; }
+  __device__ __forceinline__ int count() const { return EPILOGUE ? 1 : g.count; }
   __device__ __forceinline__ int units() const { return g.units; }
   __device__ __forceinline__ int cols() const { return g.cols; }
   __device__ __forceinline__ bool bf16() const { return DT == DT_BF16; }
-  __device__ __forceinline__ const Problem& problem(int) const { return g.p; }
-  __device__ __forceinline__ const CUtensorMap* map_a(int) const { return &g.ta; }
-  __device__ __forceinline__ const CUtensorMap* map_b(int) const { return &g.tb; }
+  __device__ __forceinline__ int index(int p) const { return EPILOGUE ? 0 : p; }
+  __device__ __forceinline__ const Problem& problem(int p) const { return g.p[index(p)]; }
+  __device__ __forceinline__ const CUtensorMap* map_a(int p) const { return &g.maps[index(p)][0]; }
+  __device__ __forceinline__ const CUtensorMap* map_b(int p) const { return &g.maps[index(p)][1]; }
   __device__ __forceinline__ const CUtensorMap* map_a_t(int) const { return nullptr; }
   __device__ __forceinline__ const CUtensorMap* map_b_t(int) const { return nullptr; }
   __device__ __forceinline__ int za(int) const { return 1; }
   __device__ __forceinline__ int zb(int) const { return 1; }
   __device__ __forceinline__ int parts(int) const { return 1; }
-  __device__ __forceinline__ Target target(int, int) const { return Target(); }
+  __device__ __forceinline__ Target target(int p, int) const { return Target{index(p)}; }
   __device__ __forceinline__ void prefetch(const Target&, const Block&, int64_t, int, int) const {}
-  __device__ __forceinline__ void finish(const Target&, const Block& b, float (&v)[32],
+  __device__ __forceinline__ void finish(const Target& t, const Block& b, float (&v)[32],
                                          int64_t row0, int col, int n, int) const {
     if constexpr (EPILOGUE) {
-      finish_linear<DT>(g.out, b, v, row0, col, n);
+      finish_linear<DT>(g.out[0], b, v, row0, col, n);
     } else {
+      const Out& o = g.out[t.p];
       row_put<DT>(b, v);
-      block_store<2>(b, g.out.out + (row0 * g.out.ld + col) * 2, g.out.ld, n);
+      block_store<2>(b, o.out + (row0 * o.ld + col) * 2, o.ld, n);
     }
   }
 };
