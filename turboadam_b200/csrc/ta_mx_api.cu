@@ -191,11 +191,36 @@ double tile_cycles(double kblocks, int cols) {
   return std::max(loop, epilogue) + 0.3 * std::min(loop, epilogue);
 }
 
-// Tile width and splits of a launch: the lowest estimate of (rounds of tiles) x (time of a tile)
-// over the widths the operands' layouts allow. Wide tiles use the tensor pipe best, narrow ones
-// give every pair of SMs a share of a small result. Where even the narrow ones do not, long sums
-// are split: the partial tiles cost about 3000 cycles and a pass over them per split.
-Shape choose(const std::vector<Product>& ps, int pairs) {
+// A split sum also costs its partial tiles' way through memory.
+double unit_cycles(const Product& p, int splits, int cols) {
+  return tile_cycles((double)cdiv(std::max<int64_t>(1, blocks_of(p)), splits), cols) +
+         (splits > 1 ? 3000.0 + splits * 2.5 * cols : 0.0);
+}
+
+// Cycles of a launch whose pair w takes units w, w + pairs, ... of the list: the most loaded
+// pair's.
+double launch_cycles(const std::vector<Product>& ps, const std::vector<int>& splits, int cols,
+                     int pairs) {
+  if (ps.size() == 1)
+    return (double)cdiv(tiles_of(ps[0], cols) * ps[0].batch * splits[0], pairs) *
+           unit_cycles(ps[0], splits[0], cols);
+  std::vector<double> load(pairs, 0.0);
+  int64_t first = 0;
+  for (size_t i = 0; i < ps.size(); ++i) {
+    const int64_t n = tiles_of(ps[i], cols) * ps[i].batch * splits[i];
+    const double c = unit_cycles(ps[i], splits[i], cols);
+    for (int w = 0; w < pairs; ++w) load[w] += (double)(n / pairs) * c;
+    for (int64_t u = 0; u < n % pairs; ++u) load[(first + u) % pairs] += c;
+    first += n;
+  }
+  return *std::max_element(load.begin(), load.end());
+}
+
+// Tile width and splits of a launch: the lowest estimate over the widths the operands' layouts
+// allow, and over some splits of its sums. Wide tiles use the tensor pipe best, narrow ones give
+// every pair of SMs a share of a small result, and split sums a share of a long one. (A layer's
+// gradients on 8192 tokens, 96 tiles of 36 blocks and 27 of 128: 63 us unsplit.)
+Shape choose(const std::vector<Product>& ps, int pairs, bool may_split = true) {
   // MN-major (or partly transposed) operands come in whole chunks of 64 rows a CTA; the tile widths
   // of a symmetric result divide its blocks of 256
   bool chunked = false, sym = false;
@@ -210,69 +235,41 @@ Shape choose(const std::vector<Product>& ps, int pairs) {
   Shape best;
   best.splits.assign(ps.size(), 1);
   double best_time = 1e300;
+  std::vector<int> splits(ps.size());
   for (int k = 0; k < n_widths; ++k) {
     const int cols = widths[k];
     int64_t units = 0;
-    double work = 0, longest = 0;
+    double work = 0;
     for (const Product& p : ps) {
       const int64_t t = tiles_of(p, cols) * p.batch;
-      const double c = tile_cycles((double)blocks_of(p), cols);
       units += t;
-      work += (double)t * c;
-      longest = std::max(longest, c);
+      work += (double)t * unit_cycles(p, 1, cols);
     }
     if (units == 0) return best;
-    double time = ps.size() == 1 ? (double)cdiv(units, pairs) * longest
-                                 : std::max(longest, work / pairs + 0.5 * longest);
-    std::vector<int> splits(ps.size(), 1);
-    if (units < pairs) {
-      // a split sum costs its partial tiles' way through memory
-      auto split_cycles = [&](const Product& p, int64_t n) {
-        return tile_cycles((double)cdiv(blocks_of(p), n), cols) +
-               (n > 1 ? 3000.0 + (double)n * 2.5 * cols : 0.0);
-      };
-      std::vector<int> tried(ps.size(), 1);
-      double split_time = 1e300;
-      if (ps.size() == 1) {
-        // the lowest (rounds of units) x (time of one)
-        for (int64_t n = 2; n <= std::min<int64_t>(16, blocks_of(ps[0]) / 2); ++n) {
-          const double t = (double)cdiv(units * n, pairs) * split_cycles(ps[0], n);
-          if (t < split_time) {
-            split_time = t;
-            tried[0] = (int)n;
-          }
-        }
-      } else {
-        // so many that each pair gets one split of the longest sums
-        const double ideal = work / pairs;
-        double split_work = 0, split_longest = 0;
-        for (size_t i = 0; i < ps.size(); ++i) {
-          const int64_t kb = blocks_of(ps[i]);
-          const double c = tile_cycles((double)kb, cols);
-          tried[i] = (int)std::max<int64_t>(
-              1, std::min<int64_t>({kb / 2, (int64_t)(c / std::max(ideal, 1.0)), (int64_t)16}));
-          const double one = split_cycles(ps[i], tried[i]);
-          split_work += (double)(tiles_of(ps[i], cols) * ps[i].batch * tried[i]) * one;
-          split_longest = std::max(split_longest, one);
-        }
-        split_time = std::max(split_longest, split_work / pairs);
-      }
+    // one product: every split; a list: units of at most a share of a pair's even load
+    const int tries = !may_split || units > 3 * pairs ? 1 : ps.size() == 1 ? 16 : 5;
+    for (int n = 1; n <= tries; ++n) {
       int64_t tiles = 0, floats = 0;
-      for (size_t i = 0; i < ps.size(); ++i)
-        if (tried[i] > 1) {
+      for (size_t i = 0; i < ps.size(); ++i) {
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, blocks_of(ps[i]) / 2));
+        int64_t want = n;
+        if (ps.size() > 1)
+          want = n == 1 ? 1
+                        : (int64_t)(unit_cycles(ps[i], 1, cols) * (n - 1) / (work / pairs) + 0.5);
+        splits[i] = (int)std::max<int64_t>(1, std::min(want, most));
+        if (splits[i] > 1) {
           const int64_t t = 2 * tiles_of(ps[i], cols) * ps[i].batch;
           tiles += t;
-          floats += t * tried[i] * kRows * cols;
+          floats += t * splits[i] * kRows * cols;
         }
-      if (split_time < time && tiles <= kSplitTiles && floats <= kSplitFloats) {
-        time = split_time;
-        splits = tried;
       }
-    }
-    if (time < best_time) {
-      best_time = time;
-      best.cols = cols;
-      best.splits = splits;
+      if (tiles > kSplitTiles || floats > kSplitFloats) continue;
+      const double time = launch_cycles(ps, splits, cols, pairs);
+      if (time < best_time) {
+        best_time = time;
+        best.cols = cols;
+        best.splits = splits;
+      }
     }
   }
   return best;
@@ -654,10 +651,9 @@ ta_status run_chain(const std::vector<Class>& classes, const ta_ortho_options* o
   int64_t most = 0;
   int widest = 0;
   for (int t = 0; t < 3; ++t) {
-    Shape shape = choose(lists[t], pairs);
-    // an application of the first iterate may sum over two parts, the others over one: no split
-    // is planned on parts that are not there
-    if (t == PH_APPLY) shape.splits.assign(classes.size(), 1);
+    // an application of the first iterate may sum over two parts, the others over one: its sums
+    // are not split
+    const Shape shape = choose(lists[t], pairs, t != PH_APPLY);
     int64_t split_tiles = 0;
     const int64_t units =
         place_products(lists[t], shape, sp.split_ws, sp.split_count, g.p[t], &split_tiles);
