@@ -640,7 +640,7 @@ ta_status run_chain(const std::vector<Class>& classes, const ta_ortho_options* o
     lists[PH_GRAM].push_back(p);
     p.a = p.b = square(c, 0);
     lists[PH_SQUARE].push_back(p);
-    p.sym = p.padded = false;
+    p.sym = false;
     p.M = c.rows;
     p.N = c.cols;
     p.a = c.tall ? iterate(c, 0, false) : square(c, 0);

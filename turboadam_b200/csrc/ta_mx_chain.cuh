@@ -154,11 +154,12 @@ struct ChainView {
   __device__ __forceinline__ void finish(const Target& t, const Block& b, float (&v)[32],
                                          int64_t row0, int col, int n, int N) const {
     if (ph.end == END_POLY) {
-      finish_half<true>(t.out, t.ld, t.aux, t.ld_aux, b, v, t.alpha, ph.c0, ph.c1, row0, col, n);
+      finish_half<true>(t.out, t.ld, t.aux, t.ld_aux, b, v, t.alpha, ph.c0, ph.c1, row0, col);
     } else if (ph.end == END_SCALE) {
-      finish_half<false>(t.out, t.ld, nullptr, 0, b, v, t.alpha, 0.f, 0.f, row0, col, n);
+      finish_half<false>(t.out, t.ld, nullptr, 0, b, v, t.alpha, 0.f, 0.f, row0, col);
     } else {
       const int dt = t.item->out_dt;
+      n = min(n, N - col);  // the result's lines are not padded
       if (dt == DT_BF16) finish_final<DT_BF16>(*t.item, b, v, t.alpha, N, row0, col, n);
       else if (dt == DT_F32) finish_final<DT_F32>(*t.item, b, v, t.alpha, N, row0, col, n);
       else finish_final<DT_F16>(*t.item, b, v, t.alpha, N, row0, col, n);

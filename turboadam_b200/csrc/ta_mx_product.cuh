@@ -238,11 +238,12 @@ __device__ __forceinline__ bool whole_lines(const void* p, int64_t ld, int n, in
   return n * size == kLine && (((uint32_t)(uintptr_t)p | (uint32_t)(ld * size)) & 15) == 0;
 }
 
-// p: the block's first element; n valid columns of SIZE bytes, lines ld elements apart.
-template <int SIZE>
+// p: the block's first element; n valid columns of SIZE bytes, lines ld elements apart. WHOLE: its
+// lines are known to be whole.
+template <int SIZE, bool WHOLE = false>
 __device__ __forceinline__ void block_load(const Block& b, const uint8_t* p, int64_t ld, int n) {
   using T = typename std::conditional<SIZE == 4, uint32_t, uint16_t>::type;
-  if (whole_lines(p, ld, n, SIZE)) {
+  if (WHOLE || whole_lines(p, ld, n, SIZE)) {
     const int r0 = b.lane >> 2;
     const int64_t step = ld * (8 * SIZE);
     const uint8_t* q = p + r0 * ld * SIZE + (b.lane & 3) * 16;
@@ -253,19 +254,26 @@ __device__ __forceinline__ void block_load(const Block& b, const uint8_t* p, int
 #pragma unroll
     for (int i = 0; i < 4; ++i) sts16(b.line + i * 8 * kLine, v[i]);
   } else {
-    const int per = 16 / SIZE * 4;  // columns of a block
-    for (int e = b.lane; e < b.rows * per; e += 32)
-      if (e % per < n)
-        sts_elem<SIZE>(b.at(e / per, e % per * SIZE),
-                       reinterpret_cast<const T*>(p)[e / per * ld + e % per]);
+    constexpr int kPer = kLine / SIZE, kStep = 32 / kPer;  // columns of a block; rows at a time
+    const int c = b.lane % kPer;
+    const T* q = reinterpret_cast<const T*>(p) + c;
+    for (int r0 = b.lane / kPer; r0 < b.rows; r0 += 8 * kStep) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = r0 + i * kStep < b.rows && c < n ? q[(r0 + i * kStep) * ld] : (T)0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i * kStep < b.rows) sts_elem<SIZE>(b.at(r0 + i * kStep, c * SIZE), v[i]);
+    }
   }
   __syncwarp();
 }
-template <int SIZE>
+template <int SIZE, bool WHOLE = false>
 __device__ __forceinline__ void block_store(const Block& b, uint8_t* p, int64_t ld, int n) {
   using T = typename std::conditional<SIZE == 4, uint32_t, uint16_t>::type;
   __syncwarp();
-  if (whole_lines(p, ld, n, SIZE)) {
+  if (WHOLE || whole_lines(p, ld, n, SIZE)) {
     const int r0 = b.lane >> 2;
     const int64_t step = ld * (8 * SIZE);
     uint8_t* q = p + r0 * ld * SIZE + (b.lane & 3) * 16;
@@ -276,11 +284,12 @@ __device__ __forceinline__ void block_store(const Block& b, uint8_t* p, int64_t 
     for (int i = 0; i < 4; ++i, q += step)
       if (r0 + 8 * i < b.rows) *reinterpret_cast<uint4*>(q) = v[i];
   } else {
-    const int per = 16 / SIZE * 4;
-    for (int e = b.lane; e < b.rows * per; e += 32)
-      if (e % per < n)
-        reinterpret_cast<T*>(p)[e / per * ld + e % per] =
-            (T)lds_elem<SIZE>(b.at(e / per, e % per * SIZE));
+    constexpr int kPer = kLine / SIZE, kStep = 32 / kPer;
+    const int c = b.lane % kPer;
+    T* q = reinterpret_cast<T*>(p) + c;
+#pragma unroll 8
+    for (int r = b.lane / kPer; r < b.rows; r += kStep)
+      if (c < n) q[r * ld] = (T)lds_elem<SIZE>(b.at(r, c * SIZE));
   }
   __syncwarp();
 }
@@ -453,14 +462,15 @@ __device__ __forceinline__ void finish_linear(const Out& o, const Block& b, floa
 }
 
 // One chunk of a Newton-Schulz matrix: the sums v of rows [row0, row0 + 32) by columns
-// [col, col + n), stored in fp16 as alpha v, or as the polynomial c0 I + c1 A + alpha v of A = aux.
+// [col, col + 32), stored in fp16 as alpha v, or as the polynomial c0 I + c1 A + alpha v of
+// A = aux. Its lines are padded to whole chunks: no ragged edge.
 template <bool POLY>
 __device__ __forceinline__ void finish_half(uint8_t* out, int64_t ld, const uint8_t* aux,
                                             int64_t ld_aux, const Block& b, float (&v)[32],
-                                            float alpha, float c0, float c1, int64_t row0, int col,
-                                            int n) {
+                                            float alpha, float c0, float c1, int64_t row0,
+                                            int col) {
   if constexpr (POLY) {
-    block_load<2>(b, aux + (row0 * ld_aux + col) * 2, ld_aux, n);
+    block_load<2, true>(b, aux + (row0 * ld_aux + col) * 2, ld_aux, 32);
     row_get<DT_F16>(b, [&](int i, float x) { v[i] = fmaf(alpha, v[i], c1 * x); });
     if (row0 == col) {  // both are multiples of 32: the diagonal is in this chunk or not
 #pragma unroll
@@ -471,7 +481,7 @@ __device__ __forceinline__ void finish_half(uint8_t* out, int64_t ld, const uint
     for (int i = 0; i < 32; ++i) v[i] *= alpha;
   }
   row_put<DT_F16>(b, v);
-  block_store<2>(b, out + (row0 * ld + col) * 2, ld, n);
+  block_store<2, true>(b, out + (row0 * ld + col) * 2, ld, 32);
 }
 
 // ---- roles -----------------------------------------------------------------------
