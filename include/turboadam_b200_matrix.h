@@ -51,10 +51,12 @@ enum {
  *   O <- X
  * The products run on fp16 operands (X, A and the polynomial, each scaled by
  * a power of two) with fp32 sums; X enters unrounded (16-bit inputs), and the
- * steps act in pairs, X <- P' P X with the second Gram matrix formed from the
- * first. The relative error is about 1.5e-3 of O; bf16 operands would leave
- * 1e-2 to 3e-2. A zero matrix gives zero; a NaN or an infinity in a matrix
- * makes all of that matrix's O NaN.
+ * first two steps (of large long matrices all steps) act in pairs, X <- P' P X
+ * with the second Gram matrix formed from the first. The relative error is
+ * about 1.5e-3 of O; bf16 operands would leave 1e-2 to 3e-2. Coefficients have
+ * to keep singular values below 8 (the quintic: 1.3), or fp16 overflows. A
+ * zero matrix gives zero; a NaN or an infinity in a matrix makes all of that
+ * matrix's O NaN.
  */
 typedef struct ta_ortho_tensor {
   const void* in_dev;
@@ -78,8 +80,8 @@ typedef struct ta_ortho_options {
 TA_API size_t ta_ortho_workspace_size(const ta_ortho_tensor* tensors, int32_t n_tensors,
                                       const ta_ortho_options* options);
 
-/* Orthogonalises (and, with TA_ORTHO_UPDATE, applies) the whole list: for every 8 distinct shapes
- * 7 launches for two steps, 3 for a last odd one, and 3 or more launches before them. */
+/* Orthogonalises (and, with TA_ORTHO_UPDATE, applies) the whole list: three or more small kernels
+ * (tables, momentum and norm, scaling), then one cooperative kernel for every 8 distinct shapes. */
 TA_API ta_status ta_orthogonalize(const ta_ortho_tensor* tensors, int32_t n_tensors,
                                   const ta_ortho_options* options, void* workspace_dev,
                                   size_t workspace_bytes, uint32_t* status_dev, void* stream);

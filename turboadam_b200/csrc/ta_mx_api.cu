@@ -45,6 +45,7 @@ inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline int64_t dt_bytes(int dt) { return dt == TA_F32 ? 4 : 2; }
 
+constexpr int64_t kMaxUnits = 0x70000000;  // work units of a launch (32-bit, with room to step)
 constexpr int64_t kMaxDim = 0x7fffff00;  // every dimension (rows, columns) is held in 32 bits
 
 constexpr int kMaxDevices = 64;
@@ -381,7 +382,7 @@ ta_status run_linear(const std::vector<Product>& ps, const std::vector<Out>& out
   memset(&g, 0, sizeof(g));
   int64_t split_tiles = 0;
   const int64_t units = place_products(ps, shape, split_ws, split_count, g.p, &split_tiles);
-  if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
+  if (units > kMaxUnits) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
   if (units == 0) return TA_OK;
   for (size_t i = 0; i < ps.size(); ++i) {
     if (ps[i].a.k > 0) {
@@ -657,7 +658,7 @@ ta_status run_chain(const std::vector<Class>& classes, const ta_ortho_options* o
     int64_t split_tiles = 0;
     const int64_t units =
         place_products(lists[t], shape, sp.split_ws, sp.split_count, g.p[t], &split_tiles);
-    if (units > 0x7fffffff) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
+    if (units > kMaxUnits) return ta_fail(TA_ERR_UNSUPPORTED, "too many tiles in one call");
     g.units[t] = (int32_t)units;
     g.cols[t] = shape.cols;
     most = std::max(most, units);
@@ -841,10 +842,10 @@ Operand operand_of(const void* p, int64_t mn, int64_t k, const Lines& l, uint16_
 ta_status run_copies(CopyArgs a, cudaStream_t stream) {
   if (a.job[0].rows == 0) std::swap(a.job[0], a.job[1]);
   if (a.job[0].rows == 0) return TA_OK;
-  const int64_t cols = std::max(a.job[0].cols, a.job[1].cols),
-                rows = std::max(a.job[0].rows, a.job[1].rows);
-  const dim3 grid((unsigned)std::min<int64_t>(cdiv(cols, kEltThreads), 64),
-                  (unsigned)std::min<int64_t>(rows, 4096), a.job[1].rows ? 2 : 1);
+  int64_t pieces = 0;
+  for (const CopyJob& j : a.job) pieces = std::max(pieces, (int64_t)j.rows * (j.ld / 8));
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(pieces, kEltThreads), 16 * sm_count()), 1,
+                  a.job[1].rows ? 2 : 1);
   return launch(k_copy_rows, grid, kEltThreads, 0, stream, a);
 }
 

@@ -279,8 +279,9 @@ __global__ void __launch_bounds__(kEltThreads)
 }
 
 // ---- operand copies --------------------------------------------------------------
-// rows x cols 16-bit elements into rows of ld elements (TMA reads rows that start on 16 bytes); up
-// to two matrices, one for each z of the grid.
+// rows x cols 16-bit elements into rows of ld (cols rounded up to 8) elements, as TMA reads rows
+// that start on 16 bytes; up to two matrices, one for each z of the grid. A thread gathers 8
+// elements, all their loads under way together, for one 16-byte store.
 struct CopyJob {
   const uint16_t* src;
   int64_t stride;
@@ -294,9 +295,19 @@ __global__ void __launch_bounds__(kEltThreads) k_copy_rows(const __grid_constant
   chain_next();
   chain_wait();
   const CopyJob& j = a.job[blockIdx.z];
-  for (int r = blockIdx.y; r < j.rows; r += gridDim.y)
-    for (int c = blockIdx.x * kEltThreads + threadIdx.x; c < j.cols; c += gridDim.x * kEltThreads)
-      j.dst[(int64_t)r * j.ld + c] = j.src[(int64_t)r * j.stride + c];
+  const int per = j.ld / 8, cols = j.cols;
+  const int64_t pieces = (int64_t)j.rows * per, step = (int64_t)gridDim.x * kEltThreads;
+  for (int64_t e = (int64_t)blockIdx.x * kEltThreads + threadIdx.x; e < pieces; e += step) {
+    const int64_t r = pieces <= 0x7fffffff ? (int64_t)((uint32_t)e / (uint32_t)per) : e / per;
+    const int c = (int)(e - r * per) * 8;
+    const uint16_t* q = j.src + r * j.stride + c;
+    uint16_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? q[k] : (uint16_t)0;
+    *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) =
+        make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16,
+                   v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
+  }
 }
 
 // ---- gradient of the activation, and of the bias -----------------------------------
