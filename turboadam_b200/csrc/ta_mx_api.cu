@@ -416,11 +416,12 @@ constexpr float kScaleX = 1024.f, kScaleA = 1024.f, kScaleP = 256.f, kScaleT = 5
 // so X is never rounded while its small singular values still drown in the error of the large
 // ones: that halves the error (2-norm, on spectra that fall by 50 within a quarter of their
 // length over a floor: 1.3e-3 against 2.0e-3; bf16 operands would leave 2e-2). A later pair
-// saves products only where r is well over 1, and rounds P and A' where X was rounded before: its
-// error falls with the side (2.8e-3, 2.2e-3 in all at sides of 512 and 1024, 1.4e-3 in the
-// tests' largest). So the later steps go in pairs ("deep") from a side of 2048 and r of 2 on
-// (14336 x 4096: 2.25 ms against 2.6), and one by one elsewhere. Three steps at once would lose
-// 1e-2.
+// saves products only where r is well over 1 and there are enough of them (1024 x 4096: 168 us
+// against 171; 2048 x 8192: 401 against 456; 14336 x 4096: 2193 against 2563), and rounds P and A'
+// where X was rounded before: its error (Frobenius norm, same spectra) nears the other's as the
+// side grows, 2.6e-3 against 2.0e-3 at 512, 2.5e-3 against 2.3e-3 at 2048, 2.44e-3 against
+// 2.38e-3 at 4096. So the later steps go in pairs ("deep") from a side of 2048 and r of 2 on, and
+// one by one elsewhere. Three steps at once would lose 1e-2.
 bool deep_pairs(int64_t side, int64_t length) { return side >= 2048 && length >= 2 * side; }
 
 struct Class {  // matrices of one shape
