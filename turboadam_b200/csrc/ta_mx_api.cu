@@ -917,8 +917,8 @@ ta_status launch_few(FewArgs& g, bool cols, int64_t room, cudaStream_t stream) {
     // enough blocks for two on every SM, by letting warps share a sum where N is small
     g.warps_n = 8;
     while (g.warps_n > 1 && cdiv(g.N, g.warps_n * kFewRows) < 2 * sms) g.warps_n /= 2;
-    return launch(k_few_rows<DT, T>, dim3((unsigned)cdiv(g.N, g.warps_n * kFewRows)), 256, 0,
-                  stream, g);
+    return launch(k_few_rows<DT, T>, dim3((unsigned)cdiv(g.N, g.warps_n * kFewRows)), 256,
+                  kFewRing, stream, g);
   }
   const int64_t blocks = cdiv(g.N, 256);
   int64_t splits = std::min<int64_t>(cdiv(4 * sms, blocks), cdiv(g.K, 32));

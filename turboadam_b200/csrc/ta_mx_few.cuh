@@ -1,11 +1,12 @@
 // ta_mx_few.cuh -- products with few rows of A (single tokens): bound by the bytes of B, which is
-// read once, straight into registers.
+// read once.
 //
 // A tile of the product engine has 256 rows; with one token its matrix instructions would work
-// on zeros, and its copies, one stage at a time and CTA pair, reach some 2.6 TB/s (45 us at
-// 4096 > 14336, bf16, for 1 to 16 tokens). Here every lane has several 16-byte loads of B under
-// way, which is what HBM asks for: 23 us for one token (5.1 TB/s), 34 us for two, 48 us for four,
-// where a lane's arithmetic takes over; beyond, the tiles are faster. Two forms, by which dimension of B is contiguous:
+// on zeros, and its copies, one stage at a time and CTA pair, reach some 3 TB/s (36 to 39 us
+// at 4096 > 14336, bf16, for 1 to 8 tokens). Here every lane has several 16-byte loads of B under
+// way, which is what HBM asks for: 21.5 us for one token (5.5 TB/s), 23 us for two, 36 us for
+// four, where a lane's arithmetic takes over (4096 > 4096: 8.6, 9.5 and 12.4 us, the tiles 24);
+// beyond, the tiles are faster. Two forms, by which dimension of B is contiguous:
 //   k_few_rows: the sum's (an output by input weight): a warp takes four rows of B;
 //   k_few_cols: the result's: a lane takes eight columns, the sum is split over the warps of a
 //               block and over blocks, and k_few_finish adds the blocks' parts in order.
@@ -18,6 +19,12 @@ namespace mx {
 
 constexpr int kFewMax = 4;   // rows of A
 constexpr int kFewRows = 4;  // rows of B a warp takes
+// Steps of a warp's copies in shared memory. Four blocks an SM with three steps each measured 23 us
+// for two tokens and 37 for four; loads into registers, one step ahead, 32 and 46 (their registers
+// leave two blocks), two steps ahead 27 and 36; three blocks with four steps 30 and 37. One token
+// takes 21.5 us from here and took 23 from registers (4096 > 4096: 8.4 and 7.7).
+constexpr int kFewStages = 3;
+constexpr size_t kFewRing = (size_t)8 * kFewStages * kFewRows * 32 * 16;  // bytes
 
 struct FewArgs {
   const uint16_t* a;  // [tokens][K], rows lda apart
@@ -55,6 +62,17 @@ __device__ __forceinline__ uint4 load_once(const uint16_t* p) {
       : "l"(p));
   return v;
 }
+__device__ __forceinline__ void copy16_async(uint4* dst, const uint16_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 template <int DT>
 __device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -68,45 +86,60 @@ __device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
 
 // Rows of both operands start on 16 bytes and K is a multiple of 8.
 template <int DT, int T>
-__global__ void __launch_bounds__(256) k_few_rows(const __grid_constant__ FewArgs g) {
+__global__ void __launch_bounds__(256, 4) k_few_rows(const __grid_constant__ FewArgs g) {
   chain_next();
   chain_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wn = warp % g.warps_n, wk = warp / g.warps_n, warps_k = 8 / g.warps_n;
   const int row0 = (blockIdx.x * g.warps_n + wn) * kFewRows;
+  extern __shared__ __align__(16) uint4 few_ring[];
   float acc[kFewRows][T] = {};
   const uint16_t* b[kFewRows];
 #pragma unroll
   for (int r = 0; r < kFewRows; ++r) b[r] = g.b + (int64_t)min(row0 + r, g.N - 1) * g.ldb;
   if (row0 < g.N) {
-    // the next step's pieces of B are under way while this one's are used
-    const int step = warps_k * 256;
-    int k = (wk * 32 + lane) * 8;
-    uint4 next[kFewRows];
-#pragma unroll
-    for (int r = 0; r < kFewRows; ++r)
-      next[r] = k < g.K ? load_once(b[r] + k) : make_uint4(0, 0, 0, 0);
-    for (; k < g.K; k += step) {
-      float x[kFewRows][8];
-#pragma unroll
-      for (int r = 0; r < kFewRows; ++r) unpack8<DT>(next[r], x[r]);
-      if (k + step < g.K) {
-#pragma unroll
-        for (int r = 0; r < kFewRows; ++r) next[r] = load_once(b[r] + k + step);
-      }
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        if (t >= g.tokens) break;
-        float y[8];
-        unpack8<DT>(*reinterpret_cast<const uint4*>(g.a + t * g.lda + k), y);
+    // a lane copies its own pieces of B's rows kFewStages - 1 steps ahead, and reads them back itself
+    uint4* ring = few_ring + warp * (kFewStages * kFewRows * 32) + lane;
+    const uint32_t step = warps_k * 256, K = g.K, k0 = wk * 256 + lane * 8;
+    const int steps = (int)((K + step - 1 - min(K + step - 1, wk * 256u)) / step);
+    auto copy = [&](int s) {
+      const uint32_t k = k0 + (uint32_t)s * step;
+      if (s < steps && k < K) {
 #pragma unroll
         for (int r = 0; r < kFewRows; ++r)
+          copy16_async(ring + (s % kFewStages * kFewRows + r) * 32, b[r] + k);
+      }
+      copy_commit();
+    };
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[r][t] = fmaf(x[r][i], y[i], acc[r][t]);
+    for (int s = 0; s < kFewStages - 1; ++s) copy(s);
+    for (int s = 0; s < steps; ++s) {
+      const uint32_t k = k0 + (uint32_t)s * step;
+      __syncwarp();  // (the stage that is filled again was read in the last step)
+      copy(s + kFewStages - 1);
+      float y[T][8];
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        unpack8<DT>(t < g.tokens && k < K ? *reinterpret_cast<const uint4*>(g.a + t * g.lda + k)
+                                          : make_uint4(0, 0, 0, 0),
+                    y[t]);
+      copy_wait<kFewStages - 1>();
+      if (k < K) {
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+          float x[8];
+          unpack8<DT>(ring[(s % kFewStages * kFewRows + r) * 32], x);
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[r][t] = fmaf(x[i], y[t][i], acc[r][t]);
+        }
       }
     }
+    copy_wait<0>();
   }
-  __shared__ float sums[8][kFewRows * T];
+  __syncthreads();  // (the sums lie where the copies did)
+  float(*sums)[kFewRows * T] = reinterpret_cast<float(*)[kFewRows * T]>(few_ring);
 #pragma unroll
   for (int r = 0; r < kFewRows; ++r)
 #pragma unroll
@@ -140,8 +173,8 @@ __global__ void __launch_bounds__(256) k_few_cols(const __grid_constant__ FewArg
   constexpr int kStretch = 1024 / T;
   __shared__ __align__(16) float xs[kStretch][T];
   float acc[T][8] = {};
-  for (int kc = k0; kc < k1; kc += kStretch) {
-    const int len = min(kStretch, k1 - kc);
+  for (int64_t kc = k0; kc < k1; kc += kStretch) {
+    const int len = (int)min((int64_t)kStretch, k1 - kc);
     __syncthreads();
     for (int e = threadIdx.x; e < len * T; e += 256) {
       const int t = e / len, k = e % len;
