@@ -262,6 +262,30 @@ def test_linear_non_finite():
         assert torch.isnan(dx[3, 0]) or act is None
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activation_over_its_range(act, dtype):
+    """Through a unit weight, so z is exact: the value is off by its rounding and some 1e-6 of itself
+    (2^-18, the exponential's relative error far out), the derivative by half a step of 2^-14 and
+    2^-20, and by its rounding as dx."""
+    from turboadam_b200 import linear_act
+
+    x = torch.cat([torch.linspace(-s, s, 40001, device="cuda") for s in (1.0, 6.0, 40.0)])
+    x = x.to(dtype).view(-1, 1).requires_grad_(True)
+    w = torch.ones(8, 1, device="cuda", dtype=dtype)
+    y = linear_act(x, w, activation=act)
+    z = x.detach().double()
+    v, d = act64(z, act)
+    want = v.expand_as(y)
+    u = U[dtype]
+    within(y.detach(), want, (u + 2.0 ** -18) * want.abs() + 2.0 ** -21 * z.abs().clamp(max=1.0)
+           + 2.0 ** -25, "y")
+    dy = torch.zeros_like(y)
+    dy[:, 3] = 1
+    dx, = torch.autograd.grad(y, x, dy)
+    within(dx, d, (2.0 ** -15 + 2.0 ** -20) * (1 + 4 * u) + 2 * u * d.abs() + 2.0 ** -25, "dx")
+
+
 def test_linear_gradient_by_differences():
     """<grad, v> against a central difference of the layer itself, in every argument.
 
