@@ -278,6 +278,15 @@ __global__ void __launch_bounds__(kEltThreads)
   }
 }
 
+// 8 elements of 16 bits that need not be aligned, zeros from the n-th on.
+__device__ __forceinline__ uint4 gather8(const uint16_t* q, int n) {
+  uint16_t v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < n ? q[k] : (uint16_t)0;
+  return make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16,
+                    v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
+}
+
 // ---- operand copies --------------------------------------------------------------
 // rows x cols 16-bit elements into rows of ld (cols rounded up to 8) elements, as TMA reads rows
 // that start on 16 bytes; up to two matrices, one for each z of the grid. A thread gathers 8
@@ -300,13 +309,8 @@ __global__ void __launch_bounds__(kEltThreads) k_copy_rows(const __grid_constant
   for (int64_t e = (int64_t)blockIdx.x * kEltThreads + threadIdx.x; e < pieces; e += step) {
     const int64_t r = pieces <= 0x7fffffff ? (int64_t)((uint32_t)e / (uint32_t)per) : e / per;
     const int c = (int)(e - r * per) * 8;
-    const uint16_t* q = j.src + r * j.stride + c;
-    uint16_t v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? q[k] : (uint16_t)0;
     *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) =
-        make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16,
-                   v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
+        gather8(j.src + r * j.stride + c, cols - c);
   }
 }
 
@@ -314,59 +318,54 @@ __global__ void __launch_bounds__(kEltThreads) k_copy_rows(const __grid_constant
 // dz = dy act'(z), rounded to the operand type for the two products that read it; the bias
 // gradient sums the unrounded dz. A thread takes 8 columns of the y-th range of rows, a block
 // neighbouring threads' columns, so that its reads run along the rows (blocks of 8 rows by 256
-// columns took 212 us at 8192 x 14336). The column sums go to part[y], which k_bias_grad adds in
+// columns took 212 us at 8192 x 14336). What it loads stays packed until it is used: 4 rows under
+// way fit the registers of enough blocks. The column sums go to part[y], which k_bias_grad adds in
 // order.
 constexpr int kDzRows = 4;  // rows whose loads are under way together
+template <int DT>
 __global__ void __launch_bounds__(kEltThreads)
-    k_dz(const void* dy, int64_t dy_stride, const int16_t* deriv, int ld_deriv, int rows, int cols,
-         int dt, uint16_t* dz, int ld_dz, float* part) {
+    k_dz(const uint16_t* dy, int64_t dy_stride, const int16_t* deriv, int ld_deriv, int rows,
+         int cols, uint16_t* dz, int ld_dz, float* part) {
   chain_next();
   chain_wait();
   const int c0 = (blockIdx.x * blockDim.x + threadIdx.x) * 8;
   if (c0 >= cols) return;
   const int r0 = (int)((int64_t)rows * blockIdx.y / gridDim.y);
   const int r1 = (int)((int64_t)rows * (blockIdx.y + 1) / gridDim.y);
-  const bool whole = c0 + 8 <= cols;
-  const bool vec = whole && dy_stride % 8 == 0 && ((uintptr_t)dy & 15) == 0;
+  const bool vec = c0 + 8 <= cols && dy_stride % 8 == 0 && ((uintptr_t)dy & 15) == 0;
   float sum[8] = {};
   for (int r = r0; r < r1; r += kDzRows) {
-    F8 g[kDzRows];
-    uint4 code[kDzRows];
+    uint4 g[kDzRows], code[kDzRows];
 #pragma unroll
     for (int q = 0; q < kDzRows; ++q) {
       const int row = min(r + q, r1 - 1);
-      const int64_t at = (int64_t)row * dy_stride + c0;
-      if (vec) {
-        g[q] = load8(dy, at, dt);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          g[q].v[k] = c0 + k < cols ? load_as_float(dy, at + k, dt) : 0.f;
-      }
+      const uint16_t* at = dy + (int64_t)row * dy_stride + c0;
+      g[q] = vec ? *reinterpret_cast<const uint4*>(at) : gather8(at, cols - c0);
       if (deriv)  // rows of ld_deriv (a multiple of 8) codes
         code[q] = *reinterpret_cast<const uint4*>(deriv + (int64_t)row * ld_deriv + c0);
     }
 #pragma unroll
     for (int q = 0; q < kDzRows; ++q) {
       if (r + q >= r1) break;
+      const uint32_t w[4] = {g[q].x, g[q].y, g[q].z, g[q].w};
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack16(w[k], DT);
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+      }
       if (deriv) {
-        const uint32_t w[4] = {code[q].x, code[q].y, code[q].z, code[q].w};
+        const uint32_t d[4] = {code[q].x, code[q].y, code[q].z, code[q].w};
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (c0 + k < cols) g[q].v[k] *= decode_deriv((int16_t)(w[k >> 1] >> (16 * (k & 1))));
+        for (int k = 0; k < 8; ++k) v[k] *= decode_deriv((int16_t)(d[k >> 1] >> (16 * (k & 1))));
       }
-      if (dz) {
-        const int64_t at = (int64_t)(r + q) * ld_dz + c0;
-        if (whole) {
-          store8(dz, at, dt, g[q]);
-        } else {
+      if (dz)  // rows of ld_dz (a multiple of 8); nothing reads the columns from cols on
+        *reinterpret_cast<uint4*>(dz + (int64_t)(r + q) * ld_dz + c0) =
+            make_uint4(pack16(v[0], v[1], DT), pack16(v[2], v[3], DT), pack16(v[4], v[5], DT),
+                       pack16(v[6], v[7], DT));
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (c0 + k < cols) store_from_float(dz, at + k, dt, g[q].v[k]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += g[q].v[k];
+      for (int k = 0; k < 8; ++k) sum[k] += v[k];
     }
   }
   if (part) {
