@@ -2,7 +2,7 @@
 // persistent kernel: a chain of phases, each a list of symmetric or general
 // products on the tile engine's roles, with a barrier over the grid between them.
 //
-// Why one kernel. Five steps are 17 dependent products. Launched one by one each
+// Why one kernel. Five steps are 16 or 17 dependent products. Launched one by one each
 // paid some 10 us at these sizes for set-up, cold instructions and descriptors,
 // the first loads and the tail (12 x 768 x 768: 262 us for 80 us of products).
 // Here tensor memory, barriers, tensor maps and code stay, and a phase costs its

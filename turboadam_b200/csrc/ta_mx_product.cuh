@@ -7,8 +7,8 @@
 // alike. A pair of SMs (cta_group::2) computes a tile of 256 rows by C columns; each SM holds 128
 // rows of A and C / 2 rows of B. Per 64 k's that is 16 KB + 64 C bytes written and as many read,
 // or 256 + C cycles of shared memory, against 2 C cycles of the tensor pipe: the two balance at
-// C = 256, the widest tile of one instruction and the default (14336 x 4096 x 4096: 327 us,
-// 1470 TFLOP/s; a pair of 128 x 128 tiles on two SMs would need 512 cycles for 256). Two
+// C = 256, the widest tile of one instruction and the default (14336 x 4096 x 4096: 319 us,
+// 1510 TFLOP/s; a pair of 128 x 128 tiles on two SMs would need 512 cycles for 256). Two
 // instructions that share A over all 512 columns of tensor memory leave shared memory a quarter
 // idle but no second accumulator, and measured 358 us there. Narrower tiles (down to 64 columns)
 // give every pair of SMs a share of a small result. Two accumulators let a tile's epilogue run
