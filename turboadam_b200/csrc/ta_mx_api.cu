@@ -192,10 +192,13 @@ double tile_cycles(double kblocks, int cols) {
   return std::max(loop, epilogue) + 0.3 * std::min(loop, epilogue);
 }
 
-// A split sum also costs its partial tiles' way through memory.
+// A split sum also costs its partial tiles' way through memory, and the last split's adding them
+// up one after another. (With a third of this cost 64 tokens of 4096 > 4096 took 25 us instead of
+// 18, 600 of 14336 > 4096 72 instead of 63 and eight GPT-2 attention matrices 252 instead of 239
+// orthogonalised; with more, a 1024 x 4096 matrix 177 instead of 169.)
 double unit_cycles(const Product& p, int splits, int cols) {
   return tile_cycles((double)cdiv(std::max<int64_t>(1, blocks_of(p)), splits), cols) +
-         (splits > 1 ? 3000.0 + splits * 2.5 * cols : 0.0);
+         (splits > 1 ? 8000.0 + splits * 12.0 * cols : 0.0);
 }
 
 // Cycles of a launch whose pair w takes units w, w + pairs, ... of the list: the most loaded
