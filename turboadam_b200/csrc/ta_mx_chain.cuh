@@ -194,10 +194,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Cta x;
   cta_begin(x, smem, g.stages, g.stage_bytes, g.status);
-  // the CTA's own barrier between phases: the first copy warp opens it
+  // the CTA's own barriers between phases: the first copy warp opens `go`, the second copy warp
+  // answers on `passed`
   const uint32_t go = x.tiles0 + kBarrierOffset + 8 * (2 * kMaxStages + 5);
+  const uint32_t passed = go + 8;
   if (threadIdx.x == 0) {
     bar_init(go, 1);
+    bar_init(passed, 1);
     bar_init_fence();
   }
   cta_meet(x);
@@ -209,15 +212,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   for (int i = 0; i < g.phases; ++i) {
     const ChainView v{g, g.phase[i]};
     const Unit w = locate(v, min(x.worker, v.units() - 1), 0);
-    // between phases: the first copy warp waits for the grid and opens the CTA's barrier
+    // Between phases: the first copy warp waits for the grid and opens the CTA's barrier. A barrier
+    // that opened twice would look closed to a warp that had yet to see the first time, so nobody
+    // may be left behind: the epilogue warps passed the last gate before this CTA arrived at the
+    // grid; the second copy warp, which has no part in that where the CTA has no unit, answers.
     auto gate = [&] {
       if (i == 0 || !r.ok) return r.ok;
       bool ok;
       if (warp == 0) {
-        ok = __all_sync(0xffffffffu, grid_wait(g, (uint32_t)i * gridDim.x));
+        ok = i == 1 || __all_sync(0xffffffffu, bar_wait(passed, (i - 2) & 1, g.status));
+        ok = ok && __all_sync(0xffffffffu, grid_wait(g, (uint32_t)i * gridDim.x));
         if (ok && lane == 0) bar_arrive_cluster(go);
       } else {
         ok = __all_sync(0xffffffffu, bar_wait(go, (i - 1) & 1, g.status));
+        if (ok && warp == 1 && lane == 0) bar_arrive_cluster(passed);
       }
       asm volatile("fence.proxy.async.global;" ::: "memory");
       return ok;
