@@ -3,7 +3,7 @@ what else the size lists of test_gpu_matrix.py do not reach. Bounds as derived t
 import pytest
 import torch
 
-from test_gpu_matrix import ORTHO_TOL, ortho64, rel
+from test_gpu_matrix import ORTHO_TOL, U, check_linear, make_linear, ortho64, rel, within
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,51 @@ def test_ortho_pairs_without_tiles():
             with torch.cuda.stream(side):
                 noise.mul_(1.0)
             assert torch.equal(orthogonalize(x, dtype=torch.float32), first)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("act", [None, "gelu", "relu"])
+@pytest.mark.parametrize("layout", ["oi", "io"])
+@pytest.mark.parametrize("tokens,fan_in", [(2, 8), (4, 768), (9, 768), (64, 768), (300, 8),
+                                           (300, 65), (1, 768)])
+def test_linear_one_output(tokens, fan_in, layout, act):
+    """A value or reward head: its weight's gradient is a product whose left operand has one row,
+    of elements that do not lie next to each other."""
+    for dtype in (torch.bfloat16, torch.float16):
+        check_linear(make_linear(tokens, fan_in, 1, dtype, layout), act)
+
+
+def test_linear_one_input():
+    """One input, the weight input by output: the weight's gradient has one row of x, here a column
+    of a wider matrix."""
+    for step, at in ((8, 0), (8, 2), (9, 2)):
+        c = make_linear(40, 1, 64, torch.bfloat16)
+        c["w"] = c["w"].reshape(1, 64).t()
+        assert c["w"].stride() == (1, 64)
+        wide = torch.randn(40, step, device="cuda").bfloat16()
+        wide[:, at:at + 1] = c["x"]
+        c["x"] = wide[:, at:at + 1]
+        check_linear(c, "silu")
+
+
+@pytest.mark.parametrize("fan_out", [64, 7])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_one_strided_token(dtype, fan_out):
+    """One token whose elements lie apart (a matrix's column, every other element), with and without
+    copies of it, against weights of both layouts."""
+    from turboadam_b200 import linear_act
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    m = torch.randn(96, 24, device="cuda", generator=g).to(dtype)
+    odd = torch.randn(96, 25, device="cuda", generator=g).to(dtype)
+    flat = torch.randn(1, 192, device="cuda", generator=g).to(dtype)
+    tokens = (m[:, 3], m[:, 8], m[:, 3:4].t(), m[:, 16:17].t(), odd[:, 5], odd.t()[:1],
+              flat[:, ::2], flat[0, 1::2])
+    for w in (torch.randn(fan_out, 96, device="cuda", generator=g).to(dtype),
+              torch.randn(96, fan_out, device="cuda", generator=g).to(dtype).t()):
+        for x in tokens:
+            y = linear_act(x, w)
+            want = x.double() @ w.double().t()
+            mag = x.double().abs() @ w.double().abs().t()
+            assert y.shape == want.shape
+            within(y, want, U[dtype] * want.abs() + 112 * 2.0 ** -22 * mag + 1e-6, "y")

@@ -905,10 +905,11 @@ ta_status check_space(const Arena& need, void* ws, size_t bytes, const uint32_t*
   return TA_OK;
 }
 
-// A few rows of A against all of B, read where they lie.
+// A few rows of A, each contiguous (the elements of an MN-major one are a line apart, of a single
+// row too), against all of B, read where they lie.
 bool few_rows(const Product& p) {
   if (p.M < 1 || p.M > kFewMax || p.a.k < 1) return false;
-  if (p.a.mn_major && p.M > 1) return false;
+  if (p.a.mn_major) return false;
   if (!aligned16(p.a.p) || (p.M > 1 && p.a.ld % 8)) return false;
   return p.b.mn_major ? p.N % 8 == 0 : p.a.k % 8 == 0;  // (B's lines start on 16 bytes)
 }
