@@ -83,3 +83,57 @@ def test_linear_one_strided_token(dtype, fan_out):
             mag = x.double().abs() @ w.double().abs().t()
             assert y.shape == want.shape
             within(y, want, U[dtype] * want.abs() + 112 * 2.0 ** -22 * mag + 1e-6, "y")
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(1, 9), (60, 90), (90, 60), (300, 500), (500, 300), (3, 40, 64),
+                                   (2, 520, 400), (1030, 1100)])
+def test_ortho_float32_input_is_a_pair(shape):
+    """One step with coefficients (1, 0, 0) returns X itself. A pair of fp16 numbers holds it to
+    2^-22, the sums may truncate at 2^-22 and three roundings to fp32 follow: 2^-20 covers them;
+    one fp16 number would leave some 2^-13."""
+    from turboadam_b200 import orthogonalize
+
+    x = torch.randn(*shape, device="cuda")
+    got = orthogonalize(x, steps=1, coefficients=(1.0, 0.0, 0.0), dtype=torch.float32)
+    want = x.double() / (x.double().square().sum((-2, -1), keepdim=True).sqrt() + 1e-7)
+    assert rel(got, want) <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("shape", [(600, 700), (700, 600), (320, 640), (1024, 1280), (1280, 520)])
+def test_ortho_low_half_of_a_pair(shape):
+    """What the low half of a 32-bit input adds: with coefficients (0, 1, 0) one step is A X, and
+    for x = hi + lo (hi an fp16 number, lo = +- 2^-12 hi by column, so that <hi, lo> = 0 and the
+    norm stays) the difference to hi's result is A lo.
+
+    A is rounded to fp16 (2^-11). The fp32 sums run over some K / 8 additions of truncated 2^-22
+    each, of a sum 2^12 times the difference: at most K 2^-13, 0.13 at K = 1024, where every one is an
+    error of full size and one sign, and a small part of that otherwise.
+    (Blocks of A read the wrong way round would leave 0.3 and more.)"""
+    from turboadam_b200 import orthogonalize
+
+    rows, cols = sorted(shape)
+    tall = shape[0] > shape[1]
+    for seed in range(100):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        half = (torch.randn(rows, 3, device="cuda", generator=g) @
+                torch.randn(3, cols // 2, device="cuda", generator=g))
+        hi = torch.cat([half, half], 1).bfloat16().double()
+        sign = torch.ones(cols, device="cuda", dtype=torch.float64)
+        sign[cols // 2:] = -1
+        lo = hi * sign * 2.0 ** -12
+        # the scale that enters in fp32 has to be one number for both
+        norms = torch.stack([hi.norm(), (hi + lo).norm()]) + 1e-7
+        scales = (1.0 / norms).float()
+        if scales[0] == scales[1]:
+            break
+    x = (hi + lo).float()
+    assert torch.equal(x.double(), hi + lo)
+
+    def step(m):
+        m = m.float().t().contiguous() if tall else m.float()
+        out = orthogonalize(m, steps=1, coefficients=(0.0, 1.0, 0.0), dtype=torch.float32)
+        return (out.t() if tall else out).double()
+
+    a = hi / norms[0]
+    assert rel(step(x) - step(hi), (a @ a.t()) @ (lo / norms[0])) <= 0.1

@@ -627,7 +627,7 @@ __device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, 
     int k0, k1;
     split_range(P, v.parts(w.p), w.split, &k0, &k1);
     if (k0 == k1) continue;  // an empty sum: the epilogue takes zeros
-    // blocks of k's up to these come transposed
+    // blocks of k's up to these come transposed, in each part of the sum
     const int a_diag = P.a_kind ? 0x7fffffff : P.a_sym ? w.m0 / kDepth : 0;
     const int b_diag = P.b_kind ? 0x7fffffff : P.b_sym ? (w.n0 & ~(kTileRows - 1)) / kDepth : 0;
     const int buf = r.count & 1;
@@ -644,7 +644,8 @@ __device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, 
         break;
       }
       tc_fence_after();
-      const bool a_mn = kb < a_diag, b_mn = kb < b_diag;
+      const int in_part = kb < P.kblocks ? kb : kb - P.kblocks;
+      const bool a_mn = in_part < a_diag, b_mn = in_part < b_diag;
       const uint32_t idesc = mma_idesc(v.bf16(), a_mn, b_mn, kTileRows, cols);
       const uint32_t step_a = mma_k_step(a_mn), step_b = mma_k_step(b_mn);
       if (elect_one()) {
