@@ -91,8 +91,10 @@ TA_API ta_status ta_orthogonalize(const ta_ortho_tensor* tensors, int32_t n_tens
  * x is [tokens][fan_in], w [fan_out][fan_in], each with one unit stride;
  * residual and y have unit column stride. Sums, bias, activation and residual
  * are in fp32, rounded once. deriv_dev (optional): receives act' of the
- * unrounded argument as round(act' * 2^14) in int16 (-32768: NaN), in rows of
- * fan_out rounded up to 8, for ta_linear_backward.
+ * unrounded argument in 16-bit codes for ta_linear_backward of the same dtype,
+ * in rows of fan_out rounded up to 8. A code is off by at most 2^-15, and
+ * relative to act' by at most 2^-9 (bf16, down to 2^-93) or 2^-12 (fp16, down
+ * to 2^-13, 2^-25 absolute beyond).
  */
 typedef struct ta_linear {
   const void* x_dev;

@@ -1,5 +1,7 @@
 """More edges of the matrix operators on the GPU: chains in which most SM pairs have no tile, and
 what else the size lists of test_gpu_matrix.py do not reach. Bounds as derived there."""
+import math
+
 import pytest
 import torch
 
@@ -137,3 +139,97 @@ def test_ortho_low_half_of_a_pair(shape):
 
     a = hi / norms[0]
     assert rel(step(x) - step(hi), (a @ a.t()) @ (lo / norms[0])) <= 0.1
+
+
+# ---------------------------------------------------------------------------
+def deriv64(z, act):
+    """act' without cancellation far out on the negative side."""
+    if act == "gelu":
+        return (0.5 * torch.special.erfc(-z / math.sqrt(2)) +
+                z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi))
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s + z * s * torch.sigmoid(-z)
+    k = 2 * math.sqrt(2 / math.pi)  # gelu_tanh: z sigmoid(k (z + 0.044715 z^3))
+    w = k * (z + 0.044715 * z ** 3)
+    s = torch.sigmoid(w)
+    return s + z * s * torch.sigmoid(-w) * k * (1 + 3 * 0.044715 * z * z)
+
+
+# what the derivative is kept to, relative: half the operand type's rounding; down to what size
+KEPT = {torch.bfloat16: (2.0 ** -9, 2.0 ** -90), torch.float16: (2.0 ** -12, 2.0 ** -13)}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act,low", [("gelu", -10.0), ("gelu_tanh", -9.0), ("silu", -60.0)])
+def test_linear_small_derivatives(act, low, dtype):
+    """Far out on the negative side act' is small, and the gradient is as exact, relative to it, as
+    elsewhere: its own error (2^-14: exponentials of arguments up to 75, themselves rounded), the
+    code it is kept in, and the two roundings of dz and dx."""
+    from turboadam_b200 import linear_act
+
+    z = torch.cat([torch.linspace(low, -2.5, 30001), torch.linspace(-4.5, -2.5, 3001)])
+    z = z.to(dtype).cuda().view(-1, 1)
+    d = deriv64(z.double(), act)
+    kept, least = KEPT[dtype]
+    z, d = z[d.abs() >= least].view(-1, 1), d[d.abs() >= least].view(-1, 1)
+    x = z.requires_grad_(True)
+    w = torch.ones(8, 1, device="cuda", dtype=dtype)
+    y = linear_act(x, w, activation=act)
+    dy = torch.zeros_like(y)
+    dy[:, 5] = 1
+    dx, = torch.autograd.grad(y, x, dy)
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 0.0  # two roundings of a subnormal
+    within(dx, d, (2 * U[dtype] + kept + 2.0 ** -14) * (1 + 4 * U[dtype]) * d.abs() + tiny, "dx")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act,bias", [("gelu", -4.0), ("gelu_tanh", -4.0), ("silu", -10.0)])
+@pytest.mark.parametrize("tokens", [1, 3, 200])
+def test_linear_gradients_of_units_far_off(tokens, act, bias, dtype):
+    """Units whose argument stays strongly negative: their bias and weight gradients relative to the
+    sums of their terms' magnitudes. z is off by (K + 16) 2^-22 of its terms and act'' / act' is at
+    most |z| + 2 there."""
+    from turboadam_b200 import linear_act
+
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    x = (torch.randn(tokens, 16, device="cuda", generator=g) * 0.25).to(dtype)
+    w = (torch.randn(24, 16, device="cuda", generator=g) * 0.05).to(dtype)
+    b = torch.full((24,), bias, device="cuda", dtype=dtype)
+    dy = (torch.rand(tokens, 24, device="cuda", generator=g) + 0.5).to(dtype)
+    w.requires_grad_(True)
+    b.requires_grad_(True)
+    y = linear_act(x, w, b, activation=act)
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    xd, wd = x.double(), w.detach().double()
+    z = xd @ wd.t() + bias
+    z_err = 32 * 2.0 ** -22 * (xd.abs() @ wd.t().abs() + abs(bias))
+    dz = dy.double() * deriv64(z, act)
+    u = U[dtype]
+    off = dz.abs() * (KEPT[dtype][0] + 2.0 ** -14 + (z.abs() + 2) * z_err)
+    want = dz.sum(0)
+    within(db, want, (off.sum(0) + (tokens + 16) * 2.0 ** -23 * dz.abs().sum(0)) * (1 + u) +
+           u * want.abs() + 2.0 ** -25, "db")
+    off = off + u * dz.abs() + 2.0 ** -25 * (dtype == torch.float16)
+    want = dz.t() @ xd
+    mag = dz.abs().t() @ xd.abs()
+    within(dw, want, (off.t() @ xd.abs() + (tokens + 16) * 2.0 ** -22 * mag) * (1 + u) +
+           u * want.abs() + 2.0 ** -25, "dw")
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_linear_gradients_at_nan(tokens, act):
+    """A NaN argument gives NaN gradients for its token and its unit's bias, and nothing else."""
+    from turboadam_b200 import linear_act
+
+    for dtype in (torch.bfloat16, torch.float16):
+        x = torch.zeros(tokens, 16, device="cuda", dtype=dtype)
+        x[1, 0] = float("nan")
+        x.requires_grad_(True)
+        w = torch.ones(8, 16, device="cuda", dtype=dtype)
+        b = torch.zeros(8, device="cuda", dtype=dtype, requires_grad=True)
+        y = linear_act(x, w, b, activation=act)
+        dx, db = torch.autograd.grad(y, (x, b), torch.ones_like(y))
+        assert torch.isnan(dx[1]).all() and torch.isnan(db).all()
+        assert torch.isfinite(dx[0]).all() and torch.isfinite(dx[2:]).all()

@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kEltThreads)
       if (deriv) {
         const uint32_t d[4] = {code[q].x, code[q].y, code[q].z, code[q].w};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= decode_deriv((int16_t)(d[k >> 1] >> (16 * (k & 1))));
+        for (int k = 0; k < 8; ++k) v[k] *= decode_deriv<DT>(d[k >> 1] >> (16 * (k & 1)) & 0xffffu);
       }
       if (dz)  // rows of ld_dz (a multiple of 8); nothing reads the columns from cols on
         *reinterpret_cast<uint4*>(dz + (int64_t)(r + q) * ld_dz + c0) =

@@ -50,7 +50,7 @@ __device__ __forceinline__ void few_store(const FewArgs& g, int t, int n, float 
   else if (g.act == ACT_GELU) activate<true>(ACT_GELU, v, &v, &d);
   else if (g.act == ACT_GELU_TANH) activate<true>(ACT_GELU_TANH, v, &v, &d);
   else if (g.act == ACT_SILU) activate<true>(ACT_SILU, v, &v, &d);
-  if (g.deriv) g.deriv[t * g.ld_deriv + n] = encode_deriv(d);
+  if (g.deriv) g.deriv[t * g.ld_deriv + n] = (int16_t)encode_deriv<DT>(d);
   if (g.aux) v += load_as_float(g.aux, t * g.ld_aux + n, DT);
   store_from_float(g.out, t * g.ldo + n, DT, v);
 }

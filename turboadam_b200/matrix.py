@@ -277,9 +277,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     once.
 
     Differentiable once in x, weight, bias and residual. For the backward pass
-    the activation's derivative is kept (16-bit fixed point, steps of 2^-14);
-    dz = dy * derivative is rounded once to the operand type for the two
-    products that read it. A weight's gradient has the weight's layout.
+    the activation's derivative is kept in 16 bits, to half of the operand
+    type's rounding relative to itself; dz = dy * derivative is rounded once to
+    the operand type for the two products that read it. A weight's gradient has the weight's layout.
     """
     if not x.is_cuda:
         _lib.require_cuda(x)
