@@ -1,0 +1,61 @@
+"""Muon's state and arguments on the CPU: what it refuses before a kernel could run on it."""
+import pytest
+import torch
+
+
+def make(*shapes, **kw):
+    from turboadam_b200 import Muon
+
+    params = [torch.nn.Parameter(torch.zeros(*s)) for s in shapes]
+    return params, Muon(params, **kw)
+
+
+def saved(*shapes):
+    params, opt = make(*shapes)
+    for p in params:
+        opt.state[p]["momentum_buffer"] = torch.ones_like(p)
+    return opt.state_dict()
+
+
+def test_load_state_dict_refuses_a_momentum_of_another_shape():
+    """Kernels write a momentum through its pointer, at the parameter's size."""
+    params, opt = make((6, 8), (4, 5))
+    opt.load_state_dict(saved((6, 8), (4, 5)))
+    assert opt.state[params[1]]["momentum_buffer"].shape == (4, 5)
+    for shapes in (((6, 8), (2, 3)), ((8, 6), (4, 5)), ((6, 8), (20,) * 2)):
+        with pytest.raises(ValueError, match="momentum"):
+            opt.load_state_dict(saved(*shapes))
+        # and nothing has changed
+        assert [tuple(opt.state[p]["momentum_buffer"].shape) for p in params] == [(6, 8), (4, 5)]
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(2, 3), torch.zeros(8, 6), torch.zeros(6, 8).double(),
+                                 torch.zeros(6, 8, device="meta"), torch.zeros(48), "text"])
+def test_step_refuses_a_momentum_that_does_not_fit(bad, monkeypatch):
+    from turboadam_b200 import muon
+
+    calls = []
+    monkeypatch.setattr(muon, "run_ortho", lambda *a: calls.append(a))
+    (p,), opt = make((6, 8))
+    p.grad = torch.ones_like(p)
+    opt.state[p]["momentum_buffer"] = bad
+    with pytest.raises((ValueError, NotImplementedError, TypeError)):
+        opt._step_device(opt.param_groups[0], p.device, [p])
+    assert not calls
+    opt.state[p]["momentum_buffer"] = torch.zeros(6, 8)
+    opt._step_device(opt.param_groups[0], p.device, [p])
+    assert len(calls) == 1
+
+
+def test_step_refuses_a_gradient_of_another_shape(monkeypatch):
+    """A parameter whose data was replaced keeps its old gradient."""
+    from turboadam_b200 import muon
+
+    calls = []
+    monkeypatch.setattr(muon, "run_ortho", lambda *a: calls.append(a))
+    (p,), opt = make((6, 8))
+    p.grad = torch.ones_like(p)
+    p.data = torch.zeros(16, 18)
+    with pytest.raises(ValueError, match="gradient"):
+        opt._step_device(opt.param_groups[0], p.device, [p])
+    assert not calls

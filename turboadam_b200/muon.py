@@ -83,9 +83,14 @@ class Muon(Optimizer):
         saved = [s.get("momentum_buffer") if isinstance(s, dict) else None
                  for s in state_dict["state"].values()]
         index = dict(zip(state_dict["state"].keys(), saved))
-        super().load_state_dict(state_dict)
         flat = [p for g in self.param_groups for p in g["params"]]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, flat):
+            m = index.get(i)
+            if m is not None and m.shape != p.shape:
+                raise ValueError(f"momentum of shape {tuple(m.shape)} for a parameter of shape "
+                                 f"{tuple(p.shape)}")
+        super().load_state_dict(state_dict)
         for i, p in zip(ids, flat):
             m = index.get(i)
             if m is not None:
@@ -115,6 +120,29 @@ class Muon(Optimizer):
                 self._step_device(group, dev, params)
         return loss
 
+    def _fitting(self, p, dev):
+        """The gradient and momentum of a parameter, as the kernels can take them: they read and
+        write all three through pointers, at the parameter's size."""
+        m, g = self.state[p].get("momentum_buffer"), p.grad
+        if g.shape != p.shape or g.device != dev:
+            raise ValueError(f"gradient {tuple(g.shape)} on {g.device} for a parameter "
+                             f"{tuple(p.shape)} on {dev}")
+        if g.dtype not in _DTYPES:
+            raise NotImplementedError(f"grad dtype {g.dtype}")
+        if m is None:
+            m = torch.zeros(p.shape, dtype=self._momentum_dtype, device=dev)
+        elif not isinstance(m, torch.Tensor):
+            raise TypeError(f"momentum_buffer is a {type(m).__name__}, not a tensor")
+        elif m.shape != p.shape or m.device != dev:
+            raise ValueError(f"momentum {tuple(m.shape)} on {m.device} for a parameter "
+                             f"{tuple(p.shape)} on {dev}")
+        elif m.dtype not in _DTYPES:
+            raise NotImplementedError(f"momentum dtype {m.dtype}")
+        if not p.is_contiguous() or not m.is_contiguous():
+            raise NotImplementedError("Muon updates contiguous parameters and momentum")
+        self.state[p]["momentum_buffer"] = m
+        return g, m
+
     def _step_device(self, group, dev, params):
         options, coeffs = ortho_options(group["ns_coefficients"], group["ns_steps"], group["eps"],
                                         group["momentum"], group["nesterov"])
@@ -128,17 +156,8 @@ class Muon(Optimizer):
                 run_ortho((_lib.TaOrthoTensor * len(part))(*part), len(part), options, dev)
             part, used = [], 0
 
-        for p in params:
-            state = self.state[p]
-            m = state.get("momentum_buffer")
-            if m is None:
-                m = torch.zeros(p.shape, dtype=self._momentum_dtype, device=dev)
-                state["momentum_buffer"] = m
-            g = p.grad
-            if g.dtype not in _DTYPES:
-                raise NotImplementedError(f"grad dtype {g.dtype}")
-            if not p.is_contiguous() or not m.is_contiguous():
-                raise NotImplementedError("Muon updates contiguous parameters and momentum")
+        # all are checked before the first is changed
+        for p, (g, m) in zip(params, [self._fitting(p, dev) for p in params]):
             if not g.is_contiguous():
                 g = g.contiguous()
             alive.append(g)
