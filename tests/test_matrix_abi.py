@@ -250,3 +250,38 @@ def test_coefficients_per_step():
     for steps in (0, 33, 2.5, True):
         with pytest.raises(ValueError):
             check_coefficients((1, 2, 3), steps)
+
+
+# ---------------------------------------------------------------------------
+# addresses that no kernel could load from: elements at their type's alignment
+@pytest.mark.parametrize("over", [
+    {"x_dev": (1 << 20) + 1}, {"w_dev": (1 << 21) + 1}, {"y_dev": (1 << 22) + 1},
+    {"residual_dev": 4097}, {"bias_dev": 4097, "bias_dtype": 1},
+    {"bias_dev": 4098, "bias_dtype": 0},
+])
+def test_linear_refuses_misaligned_elements(lib, over):
+    op = _linear(**over)
+    rc = lib.ta_linear_forward(ctypes.byref(op), 1 << 23, 1 << 40, 1 << 10, None)
+    assert rc == ALIGN, lib.ta_last_error()
+    assert lib.ta_last_error()
+
+
+@pytest.mark.parametrize("over", [
+    {"dy_dev": (1 << 20) + 1}, {"x_dev": (1 << 21) + 1}, {"w_dev": (1 << 22) + 1},
+    {"dx_dev": (1 << 23) + 1}, {"dw_dev": (1 << 24) + 1}, {"db_dev": 4097, "bias_dtype": 2},
+    {"db_dev": 4098, "bias_dtype": 0},
+])
+def test_linear_backward_refuses_misaligned_elements(lib, over):
+    op = _grad(**over)
+    rc = lib.ta_linear_backward(ctypes.byref(op), 1 << 25, 1 << 40, 1 << 10, None)
+    assert rc == ALIGN, lib.ta_last_error()
+
+
+def test_misaligned_status_word(lib):
+    op, grad = _linear(), _grad()
+    t, o = _ortho()
+    for status in ((1 << 10) + 1, (1 << 10) + 2):
+        assert lib.ta_linear_forward(ctypes.byref(op), 1 << 23, 1 << 40, status, None) == ALIGN
+        assert lib.ta_linear_backward(ctypes.byref(grad), 1 << 25, 1 << 40, status, None) == ALIGN
+        assert lib.ta_orthogonalize(t, 1, ctypes.byref(o), 1 << 20, 1 << 40, status,
+                                    None) == ALIGN

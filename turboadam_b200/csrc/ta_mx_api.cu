@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -44,6 +45,15 @@ inline int64_t up32(int64_t x) { return (x + 31) & ~(int64_t)31; }
 inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline int64_t dt_bytes(int dt) { return dt == TA_F32 ? 4 : 2; }
+
+// Elements of the type can be loaded from there (a null pointer passes).
+bool typed(const void* p, int dt) { return (uintptr_t)p % dt_bytes(dt) == 0; }
+ta_status check_typed(std::initializer_list<std::pair<const char*, const void*>> ps, int dt) {
+  for (const auto& p : ps)
+    if (!typed(p.second, dt))
+      return ta_fail(TA_ERR_ALIGN, std::string(p.first) + " not aligned to its type");
+  return TA_OK;
+}
 
 constexpr int64_t kMaxUnits = 0x70000000;  // work units of a launch (32-bit, with room to step)
 constexpr int64_t kMaxDim = 0x7fffff00;  // every dimension (rows, columns) is held in 32 bits
@@ -474,8 +484,8 @@ ta_status plan_ortho(const ta_ortho_tensor* ts, int32_t n, const ta_ortho_option
     for (int dt : {t.in_dtype, t.out_dtype, t.momentum_dev ? t.momentum_dtype : (int)TA_F32})
       if (dt != TA_F32 && dt != TA_BF16 && dt != TA_F16)
         return bad("dtypes must be TA_F32, TA_BF16 or TA_F16");
-    if ((uintptr_t)t.in_dev % dt_bytes(t.in_dtype) || (uintptr_t)t.out_dev % dt_bytes(t.out_dtype) ||
-        (t.momentum_dev && (uintptr_t)t.momentum_dev % dt_bytes(t.momentum_dtype)))
+    if (!typed(t.in_dev, t.in_dtype) || !typed(t.out_dev, t.out_dtype) ||
+        (t.momentum_dev && !typed(t.momentum_dev, t.momentum_dtype)))
       return ta_fail(TA_ERR_ALIGN,
                      "matrix " + std::to_string(i) + ": pointer not aligned to its type");
     const bool pair = (t.flags & TA_ORTHO_PAIR) && t.in_dtype == TA_F32;
@@ -877,6 +887,9 @@ ta_status prepare_linear(const ta_linear* op, Lines* x, Lines* w) {
   if (!half_type(op->dtype)) return ta_fail(TA_ERR_INVALID, "dtype must be TA_BF16 or TA_F16");
   if (op->bias_dev && !any_type(op->bias_dtype))
     return ta_fail(TA_ERR_INVALID, "bias_dtype must be TA_F32, TA_BF16 or TA_F16");
+  MX_OK(check_typed({{"x", op->x_dev}, {"w", op->w_dev}, {"y", op->y_dev},
+                     {"residual", op->residual_dev}}, op->dtype));
+  if (op->bias_dev) MX_OK(check_typed({{"bias", op->bias_dev}}, op->bias_dtype));
   if (op->activation < TA_ACT_NONE || op->activation > TA_ACT_SILU)
     return ta_fail(TA_ERR_INVALID, "unknown activation");
   if (!lines_of(op->x_dev, op->tokens, op->fan_in, op->x_strides[0], op->x_strides[1], x))
@@ -902,6 +915,7 @@ ta_status check_space(const Arena& need, void* ws, size_t bytes, const uint32_t*
                                          std::to_string(need.used) + " are needed");
   if ((uintptr_t)ws % 256) return ta_fail(TA_ERR_ALIGN, "workspace not 256-byte aligned");
   if (!status) return ta_fail(TA_ERR_INVALID, "null status word");
+  if ((uintptr_t)status % 4) return ta_fail(TA_ERR_ALIGN, "status word not 4-byte aligned");
   return TA_OK;
 }
 
@@ -993,6 +1007,9 @@ ta_status prepare_grad(const ta_linear_grad* op, GradLines* g) {
   if (!half_type(op->dtype)) return ta_fail(TA_ERR_INVALID, "dtype must be TA_BF16 or TA_F16");
   if (op->db_dev && !any_type(op->bias_dtype))
     return ta_fail(TA_ERR_INVALID, "bias_dtype must be TA_F32, TA_BF16 or TA_F16");
+  MX_OK(check_typed({{"dy", op->dy_dev}, {"x", op->x_dev}, {"w", op->w_dev}, {"dx", op->dx_dev},
+                     {"dw", op->dw_dev}}, op->dtype));
+  if (op->db_dev) MX_OK(check_typed({{"db", op->db_dev}}, op->bias_dtype));
   const bool work = op->tokens > 0 && op->fan_out > 0;
   if (work && !op->dy_dev) return ta_fail(TA_ERR_INVALID, "null dy");
   if (op->tokens > 1 && op->dy_stride < op->fan_out)
