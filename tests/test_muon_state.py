@@ -59,3 +59,23 @@ def test_step_refuses_a_gradient_of_another_shape(monkeypatch):
     with pytest.raises(ValueError, match="gradient"):
         opt._step_device(opt.param_groups[0], p.device, [p])
     assert not calls
+
+
+def test_step_raises_version_counters(monkeypatch):
+    """The kernels write behind autograd's back; a backward pass through a graph that saved the
+    parameter before the step has to notice, as with torch's own optimizers."""
+    from turboadam_b200 import muon
+
+    monkeypatch.setattr(muon, "run_ortho", lambda *a: None)
+    (p, q), opt = make((6, 8), (4, 5))
+    x = torch.ones(3, 8, requires_grad=True)
+    loss = (x @ p.t()).sum()
+    p.grad = torch.ones_like(p)
+    opt._step_device(opt.param_groups[0], p.device, [p])
+    m = opt.state[p]["momentum_buffer"]
+    before = m._version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    opt._step_device(opt.param_groups[0], p.device, [p])
+    assert m._version > before
+    assert q._version == 0

@@ -157,7 +157,8 @@ class Muon(Optimizer):
             part, used = [], 0
 
         # all are checked before the first is changed
-        for p, (g, m) in zip(params, [self._fitting(p, dev) for p in params]):
+        fitting = [self._fitting(p, dev) for p in params]
+        for p, (g, m) in zip(params, fitting):
             if not g.is_contiguous():
                 g = g.contiguous()
             alive.append(g)
@@ -176,3 +177,6 @@ class Muon(Optimizer):
             part.append(t)
             used += need
         flush()
+        # written through pointers: graphs that saved them before the step notice
+        torch.autograd.graph.increment_version(params)
+        torch.autograd.graph.increment_version([m for _, m in fitting])
