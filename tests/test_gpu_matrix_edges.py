@@ -233,3 +233,47 @@ def test_linear_gradients_at_nan(tokens, act):
         dx, db = torch.autograd.grad(y, (x, b), torch.ones_like(y))
         assert torch.isnan(dx[1]).all() and torch.isnan(db).all()
         assert torch.isfinite(dx[0]).all() and torch.isfinite(dx[2:]).all()
+
+
+# ---------------------------------------------------------------------------
+def test_forward_mode_is_refused():
+    """A tangent must not be lost without a word, in any argument."""
+    from turboadam_b200 import linear_act, orthogonalize
+    import torch.autograd.forward_ad as fwd
+
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    args = dict(x=torch.randn(4, 16, **bf), weight=torch.randn(8, 16, **bf),
+                bias=torch.randn(8, **bf), residual=torch.randn(4, 8, **bf))
+    for name in args:
+        for grad in (False, True):
+            with fwd.dual_level():
+                dual = fwd.make_dual(args[name], torch.ones_like(args[name]))
+                other = "x" if name != "x" else "weight"
+                kw = {**args, name: dual, other: args[other].clone().requires_grad_(grad)}
+                with pytest.raises(NotImplementedError, match="forward"):
+                    linear_act(**kw)
+    with fwd.dual_level():
+        m = torch.randn(6, 9, device="cuda")
+        with pytest.raises(NotImplementedError):
+            orthogonalize(fwd.make_dual(m, torch.ones_like(m)))
+        # without a tangent both run as ever
+        assert orthogonalize(m).shape == (6, 9)
+        assert linear_act(**args).shape == (4, 8)
+
+
+def test_function_transforms_are_loud():
+    """torch.func's transforms hand over tensors without storage."""
+    from turboadam_b200 import linear_act, orthogonalize
+
+    x = torch.randn(3, 4, 16, device="cuda").bfloat16()
+    w = torch.randn(8, 16, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: linear_act(t, w))(x)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: linear_act(t, w), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(orthogonalize)(x)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(orthogonalize, (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: linear_act(t, w).float().sum())(x)

@@ -15,6 +15,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -84,6 +85,13 @@ def ortho_options(coefficients, steps, eps, momentum=0.0, nesterov=False):
                                float(eps), float(momentum)), arr
 
 
+def _no_tangents(what, *tensors):
+    """The operators read data pointers, past a forward-mode tangent."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: forward-mode derivatives are not built")
+
+
 class _On:
     """``with _On(index):`` the calls inside see that device as the current one."""
 
@@ -141,9 +149,13 @@ def orthogonalize(x: torch.Tensor, steps: int = NS_STEPS, coefficients=NS_COEFFI
     unrounded, a 32-bit one as a pair of fp16 numbers; the result is within
     about 1.5e-3 of the exact iteration (2-norm), so float32 outputs carry about
     nine good bits. A zero matrix gives zero; a matrix with a NaN or an
-    infinity gives NaN throughout. Not differentiable.
+    infinity gives NaN throughout. Not differentiable: the result is detached
+    from an x that requires a gradient, and an x with a forward-mode tangent is
+    refused.
     """
     _lib.require_cuda(x)
+    if forward_ad._current_level >= 0:
+        _no_tangents("orthogonalize", x)
     if x.dim() < 2:
         raise ValueError(f"orthogonalize takes matrices, got {x.dim()} dimension(s)")
     if x.dtype not in _DTYPES or dtype not in _DTYPES:
@@ -276,7 +288,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     be float32. Sums, bias, activation and residual are in fp32 and rounded
     once.
 
-    Differentiable once in x, weight, bias and residual. For the backward pass
+    Differentiable once in x, weight, bias and residual, in reverse mode. For the backward pass
     the activation's derivative is kept in 16 bits, to half of the operand
     type's rounding relative to itself; dz = dy * derivative is rounded once to
     the operand type for the two products that read it. A weight's gradient has the weight's layout.
@@ -311,6 +323,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         if residual.shape != shape:
             raise ValueError(f"residual has shape {tuple(residual.shape)}, wanted {shape}")
         grad = grad or residual.requires_grad
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear_act", x, weight, bias, residual)
     flat = x.dim() == 2
     if not flat:
         tokens = math.prod(x.shape[:-1])
