@@ -79,3 +79,46 @@ def test_step_raises_version_counters(monkeypatch):
     opt._step_device(opt.param_groups[0], p.device, [p])
     assert m._version > before
     assert q._version == 0
+
+
+BAD = [dict(lr=-1.0), dict(lr=float("nan")), dict(momentum=1.0), dict(momentum=-0.1),
+       dict(weight_decay=-0.1), dict(adjust_lr_fn="match_rms"), dict(ns_steps=0), dict(eps=-1.0),
+       dict(ns_coefficients=(1.0, 2.0))]
+
+
+@pytest.mark.parametrize("bad", BAD)
+def test_values_of_a_group_are_checked(bad):
+    from turboadam_b200 import Muon
+
+    p, q = (torch.nn.Parameter(torch.zeros(4, 5)) for _ in range(2))
+    with pytest.raises(ValueError):
+        Muon([dict(params=[p], **bad)])
+    opt = Muon([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[q], **bad))
+    assert [g["params"] for g in opt.param_groups] == [[p]]
+
+
+def test_refused_group_is_not_added():
+    from turboadam_b200 import Muon
+
+    p, q = torch.nn.Parameter(torch.zeros(4, 5)), torch.nn.Parameter(torch.zeros(4))
+    opt = Muon([p])
+    with pytest.raises(ValueError, match="TurboAdam"):
+        opt.add_param_group(dict(params=[q]))
+    assert [g["params"] for g in opt.param_groups] == [[p]]
+    opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, 3))], lr=0.5,
+                             adjust_lr_fn="match_rms_adamw"))
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.5]
+
+
+def test_unknown_adjustment_set_later_is_refused(monkeypatch):
+    """A schedule or a loaded state may write into a group."""
+    from turboadam_b200 import muon
+
+    monkeypatch.setattr(muon, "run_ortho", lambda *a: None)
+    (p,), opt = make((6, 8))
+    p.grad = torch.ones_like(p)
+    opt.param_groups[0]["adjust_lr_fn"] = "match_rms"
+    with pytest.raises(ValueError, match="adjust_lr_fn"):
+        opt._step_device(opt.param_groups[0], p.device, [p])

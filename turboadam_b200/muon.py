@@ -20,10 +20,27 @@ from .matrix import _DTYPES, NS_COEFFICIENTS, NS_EPS, NS_STEPS, ortho_options, r
 WORKSPACE_LIMIT = 4 << 30
 
 
+def _check_adjustment(kind):
+    if kind not in (None, "original", "match_rms_adamw"):
+        raise ValueError(f"adjust_lr_fn must be 'original' or 'match_rms_adamw', got {kind!r}")
+
+
 def _gain(kind, lr, rows, cols):
-    if kind in (None, "original"):
-        return lr * math.sqrt(max(1.0, rows / cols))
-    return lr * 0.2 * math.sqrt(max(rows, cols))  # match_rms_adamw
+    if kind == "match_rms_adamw":
+        return lr * 0.2 * math.sqrt(max(rows, cols))
+    return lr * math.sqrt(max(1.0, rows / cols))
+
+
+def _check_group(group):
+    lr, momentum, decay = group["lr"], group["momentum"], group["weight_decay"]
+    if not lr >= 0:
+        raise ValueError(f"lr must not be negative, got {lr}")
+    if not 0 <= momentum < 1:
+        raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+    if not decay >= 0:
+        raise ValueError(f"weight_decay must not be negative, got {decay}")
+    _check_adjustment(group["adjust_lr_fn"])
+    ortho_options(group["ns_coefficients"], group["ns_steps"], group["eps"])  # checks them
 
 
 class Muon(Optimizer):
@@ -53,30 +70,27 @@ class Muon(Optimizer):
                  ns_coefficients=NS_COEFFICIENTS, eps: float = NS_EPS, ns_steps: int = NS_STEPS,
                  adjust_lr_fn: str | None = None, *,
                  momentum_dtype: torch.dtype = torch.float32):
-        if not lr >= 0:
-            raise ValueError(f"lr must not be negative, got {lr}")
-        if not 0 <= momentum < 1:
-            raise ValueError(f"momentum must be in [0, 1), got {momentum}")
-        if not weight_decay >= 0:
-            raise ValueError(f"weight_decay must not be negative, got {weight_decay}")
-        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
-            raise ValueError(f"adjust_lr_fn must be 'original' or 'match_rms_adamw', got "
-                             f"{adjust_lr_fn!r}")
         if momentum_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("momentum_dtype must be float32 or bfloat16, got "
                              f"{momentum_dtype}")
-        ortho_options(ns_coefficients, ns_steps, eps)  # checks them
         self._momentum_dtype = momentum_dtype
-        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum,
-                                      nesterov=nesterov, ns_coefficients=ns_coefficients, eps=eps,
-                                      ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn))
+        defaults = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                        ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps,
+                        adjust_lr_fn=adjust_lr_fn)
+        _check_group(defaults)
+        super().__init__(params, defaults)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                raise ValueError("Muon updates matrices; a parameter has "
-                                 f"{p.dim()} dimension(s): give it to TurboAdam")
+        try:
+            _check_group(self.param_groups[-1])
+            for p in self.param_groups[-1]["params"]:
+                if p.dim() < 2:
+                    raise ValueError("Muon updates matrices; a parameter has "
+                                     f"{p.dim()} dimension(s): give it to TurboAdam")
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
         """torch casts state to the parameters' dtype; the momentum keeps its own."""
@@ -144,6 +158,7 @@ class Muon(Optimizer):
         return g, m
 
     def _step_device(self, group, dev, params):
+        _check_adjustment(group["adjust_lr_fn"])
         options, coeffs = ortho_options(group["ns_coefficients"], group["ns_steps"], group["eps"],
                                         group["momentum"], group["nesterov"])
         lr = float(group["lr"])
