@@ -122,3 +122,21 @@ def test_unknown_adjustment_set_later_is_refused(monkeypatch):
     opt.param_groups[0]["adjust_lr_fn"] = "match_rms"
     with pytest.raises(ValueError, match="adjust_lr_fn"):
         opt._step_device(opt.param_groups[0], p.device, [p])
+
+
+def test_copies_and_pickles_keep_the_momentum_dtype():
+    """torch's optimizers carry defaults, state and groups over a deepcopy or a pickle only."""
+    import copy
+    import pickle
+
+    (p,), opt = make((6, 8), lr=0.5, momentum_dtype=torch.bfloat16)
+    opt.state[p]["momentum_buffer"] = torch.ones(6, 8, dtype=torch.bfloat16)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        q = other.param_groups[0]["params"][0]
+        q.grad = torch.ones_like(q)
+        assert other._fitting(q, q.device)[1].dtype == torch.bfloat16
+        del other.state[q]["momentum_buffer"]
+        assert other._fitting(q, q.device)[1].dtype == torch.bfloat16
+        assert other.param_groups[0]["lr"] == 0.5
+        other.load_state_dict(opt.state_dict())
+        assert other.state[q]["momentum_buffer"].dtype == torch.bfloat16

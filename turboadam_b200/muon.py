@@ -80,6 +80,9 @@ class Muon(Optimizer):
         _check_group(defaults)
         super().__init__(params, defaults)
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "_momentum_dtype": self._momentum_dtype}
+
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         try:
