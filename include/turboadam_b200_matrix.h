@@ -7,9 +7,10 @@
  * (ta_last_error has the message). A call enqueues kernels (and one memset)
  * only, so it can be captured into a CUDA graph. A workspace needs no set-up
  * and holds nothing between calls; calls that can overlap need workspaces of
- * their own. status_dev is a 4-byte device word the caller zeroes once and may
- * share between calls (ta_read_status takes its address): a bounded wait that
- * ran out sets TA_STATUS_WAIT_TIMEOUT in it, and the call's results are void.
+ * their own. status_dev is a 4-byte word the caller zeroes once and may share
+ * between calls, in device memory (ta_read_status takes its address) or in
+ * pinned host memory: a bounded wait that ran out sets TA_STATUS_WAIT_TIMEOUT
+ * in it, and the call's results are void.
  *
  * None of the three has a counterpart in the reference (davidkny22/turboadam),
  * which updates every tensor elementwise.

@@ -277,3 +277,35 @@ def test_function_transforms_are_loud():
         torch.func.jvp(orthogonalize, (x,), (x,))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: linear_act(t, w).float().sum())(x)
+
+
+# ---------------------------------------------------------------------------
+def test_void_results_are_reported_by_the_next_call():
+    """A wait that runs out (here the library's self-test, on the operators' own status word: a
+    kernel whose copies never come, for 1 ms) makes the following calls raise until the status has
+    been read, without a synchronisation of theirs."""
+    from turboadam_b200 import Muon, _lib, linear_act, matrix, orthogonalize
+
+    x = torch.randn(40, 16, device="cuda").bfloat16()
+    w = torch.randn(8, 16, device="cuda").bfloat16()
+    p = torch.nn.Parameter(torch.randn(16, 24, device="cuda"))
+    p.grad = torch.randn_like(p)
+    opt = Muon([p])
+    opt.step()
+    before = p.detach().clone()
+    y = linear_act(x, w)
+    out = torch.zeros(2, dtype=torch.int64, device="cuda")
+    index = torch.cuda.current_device()
+    lib = _lib.load()
+    _lib.check(lib.ta_selftest_wait_timeout(1_000_000, matrix._word(index), out.data_ptr(),
+                                            _lib.stream_ptr(index)), "self-test")
+    torch.cuda.synchronize()
+    for call in (lambda: linear_act(x, w), lambda: orthogonalize(p.detach()), opt.step):
+        for _ in range(2):
+            with pytest.raises(_lib.TurboAdamBackendError, match="void"):
+                call()
+    assert torch.equal(p.detach(), before)
+    assert matrix.read_status(clear=False) == _lib.TA_STATUS_WAIT_TIMEOUT
+    assert matrix.read_status() == _lib.TA_STATUS_WAIT_TIMEOUT
+    assert matrix.read_status() == 0
+    assert torch.equal(linear_act(x, w), y)

@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import threading
 
 import torch
 from torch.autograd import forward_ad
@@ -30,36 +31,42 @@ _ACTIVATIONS = {None: _lib.TA_ACT_NONE, "none": _lib.TA_ACT_NONE, "relu": _lib.T
                 "gelu": _lib.TA_ACT_GELU, "gelu_tanh": _lib.TA_ACT_GELU_TANH,
                 "silu": _lib.TA_ACT_SILU}
 
-_status = {}  # device index -> int32 [1], OR-ed into by every call on that device
-_words = {}   # device index -> its address
+# device index -> status word that every call on that device ORs into, and the tensor that holds it.
+# It lies in pinned host memory, which kernels reach at the same address: they write it only when a
+# wait has run out, and a call sees what earlier ones have left there without synchronising.
+_words = {}
+_words_lock = threading.Lock()
 
 
 def _word(index: int) -> int:
-    """Address of the device's status word, zeroed before any stream uses it."""
+    """Address of the device's status word. Raises if an earlier call's results are void."""
     at = _words.get(index)
     if at is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first call on a device must run outside CUDA graph capture")
-        st = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
-        torch.cuda.synchronize(index)
-        _status[index] = st
-        at = _words[index] = st.data_ptr()
-    return at
+        with _words_lock:
+            if index not in _words:
+                st = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                _words[index] = ctypes.c_uint32.from_address(st.data_ptr()), st
+            at = _words[index]
+    if at[0].value:
+        raise _lib.TurboAdamBackendError(
+            f"a bounded wait of an earlier call on cuda:{index} ran out (status "
+            f"{at[0].value:#x}): its results are void. matrix.read_status() clears this")
+    return at[1].data_ptr()
 
 
 def read_status(clear: bool = True) -> int:
     """Device status bits of the matrix operators since the last read, over
     all devices (TA_STATUS_WAIT_TIMEOUT: a bounded wait ran out and that
-    call's results are void). Synchronises."""
-    lib = _lib.load()
+    call's results are void; calls raise until the bit has been cleared).
+    Synchronises."""
     out = 0
-    for idx, st in _status.items():
-        v = ctypes.c_uint32(0)
-        with torch.cuda.device(idx):
-            torch.cuda.synchronize(idx)
-            _lib.check(lib.ta_read_status(st.data_ptr(), int(clear), ctypes.byref(v),
-                                          _lib.stream_ptr(idx)), "ta_read_status")
-        out |= v.value
+    for idx, (word, _) in list(_words.items()):
+        torch.cuda.synchronize(idx)
+        out |= word.value
+        if clear:
+            word.value = 0
     return out
 
 
@@ -122,8 +129,9 @@ def _call(size_fn, fn, what, args, dev):
             if why:
                 raise _lib.TurboAdamBackendError(
                     f"{what} failed: {why.decode(errors='replace')}")
+        word = _word(index)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = fn(*args, ws.data_ptr(), need, _word(index), torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(*args, ws.data_ptr(), need, word, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)
 
