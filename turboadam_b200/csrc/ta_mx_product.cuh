@@ -669,6 +669,9 @@ __device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, 
     // blocks of k's up to these come transposed, in each part of the sum
     const int a_diag = P.a_kind ? 0x7fffffff : P.a_sym ? w.m0 / kDepth : 0;
     const int b_diag = P.b_kind ? 0x7fffffff : P.b_sym ? (w.n0 & ~(kTileRows - 1)) / kDepth : 0;
+    int kblocks = P.kblocks;
+    asm volatile("" : "+r"(kblocks));  // (read once, not in the loop)
+    int k = k0 < kblocks ? k0 : k0 - kblocks;  // in its part
     const int buf = r.count & 1;
     const uint32_t d = x.tmem + buf * (kTmemCols / 2);
     if (!__all_sync(0xffffffffu,
@@ -683,8 +686,7 @@ __device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, 
         break;
       }
       tc_fence_after();
-      const int in_part = kb < P.kblocks ? kb : kb - P.kblocks;
-      const bool a_mn = in_part < a_diag, b_mn = in_part < b_diag;
+      const bool a_mn = k < a_diag, b_mn = k < b_diag;
       const uint32_t idesc = mma_idesc(v.bf16(), a_mn, b_mn, kTileRows, cols);
       const uint32_t step_a = mma_k_step(a_mn), step_b = mma_k_step(b_mn);
       if (elect_one()) {
@@ -699,6 +701,7 @@ __device__ __forceinline__ void mma_units(const View& v, const Cta& x, Ring& r, 
       }
       __syncwarp();
       r.next(x.stages);
+      if (++k == kblocks) k = 0;
     }
     ++r.count;
   }
