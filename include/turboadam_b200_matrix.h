@@ -51,11 +51,15 @@ enum {
  *   A <- X X^T (X^T X if rows > cols);  X <- (a I + b A + c A^2) X
  *   O <- X
  * The products run on fp16 operands (X, A and the polynomial, each scaled by
- * a power of two) with fp32 sums; X enters unrounded (16-bit inputs), and the
+ * a power of two) with fp32 sums; X enters unrounded (16-bit inputs) or to 22
+ * bits, of which the first A sees 11 (TA_ORTHO_PAIR), and the
  * first two steps (of large long matrices all steps) act in pairs, X <- P' P X
  * with the second Gram matrix formed from the first. The relative error is
- * about 1.5e-3 of O; bf16 operands would leave 1e-2 to 3e-2. Coefficients have
- * to keep singular values below 8 (the quintic: 1.3), or fp16 overflows. A
+ * 0.8e-3 to 2e-3 of O (Frobenius norm; 1.5e-3 to 5e-3 in the 2-norm; more for
+ * matrices of a few rows close to singular); bf16 operands would leave 1e-2
+ * to 3e-2. Coefficients have to keep singular values below 8 (the quintic: 1.3)
+ * and a step's polynomial and the product of a pair's below 255 (the quintic:
+ * 12), or fp16 overflows and O is NaN. A
  * zero matrix gives zero; a NaN or an infinity in a matrix makes all of that
  * matrix's O NaN.
  */

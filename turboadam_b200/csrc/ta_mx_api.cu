@@ -425,16 +425,19 @@ constexpr float kScaleX = 1024.f, kScaleA = 1024.f, kScaleP = 256.f, kScaleT = 5
 // Two steps can go as a pair. With A the Gram matrix of X, P and P' the polynomials of the steps,
 //   T = P A,  A' = P T  (the Gram matrix of P X, without forming P X),  Q = P' P,  X <- Q X:
 // in units of a side^3 product and with r = long / short side, 3 r + 5 for two steps against
-// 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the unrounded input,
-// so X is never rounded while its small singular values still drown in the error of the large
-// ones: that halves the error (2-norm, on spectra that fall by 50 within a quarter of their
-// length over a floor: 1.3e-3 against 2.0e-3; bf16 operands would leave 2e-2). A later pair
-// saves products only where r is well over 1 and there are enough of them (1024 x 4096: 168 us
-// against 171; 2048 x 8192: 401 against 456; 14336 x 4096: 2193 against 2563), and rounds P and A'
-// where X was rounded before: its error (Frobenius norm, same spectra) nears the other's as the
-// side grows, 2.6e-3 against 2.0e-3 at 512, 2.5e-3 against 2.3e-3 at 2048, 2.44e-3 against
-// 2.38e-3 at 4096. So the later steps go in pairs ("deep") from a side of 2048 and r of 2 on, and
-// one by one elsewhere. Three steps at once would lose 1e-2.
+// 6 r + 2 one by one (symmetric results at half cost). The first pair acts on the input as it is
+// held (16-bit inputs exactly, 32-bit ones to 22 bits, of which A sees the upper 11), so X is not
+// rounded while its small singular values still drown in the error of the large ones: that leaves
+// two thirds of the error (Frobenius norm against the exact iteration, on spectra that fall by 50
+// within a quarter of their length over a floor: 1.0e-3 against 1.5e-3 at 768 x 768, 1.48e-3
+// against 2.15e-3 at 1024 x 4096; bf16 operands would leave 2e-2). A later pair saves products only
+// where r is well over 1 and there are enough of them (1024 x 4096: 175 us against 177; 2048 x
+// 8192: 408 against 462; 14336 x 4096: 2209 against 2584), and rounds P and A' where X was rounded
+// before: its error nears the other's as the side grows, 2.04e-3 against 1.27e-3 at 512 x 2048, 1.97e-3
+// against 1.48e-3 at 1024 x 4096, 1.90e-3 against 1.65e-3 at 2048 x 8192, 1.83e-3 against 1.76e-3
+// at 14336 x 4096 (in the 2-norm 4.5e-3 against 2.2e-3 at 2048 x 8192). So the later steps go in
+// pairs ("deep") from a side of 2048 and r of 2 on, and one by one elsewhere. Three steps at once
+// would lose 1e-2.
 bool deep_pairs(int64_t side, int64_t length) { return side >= 2048 && length >= 2 * side; }
 
 struct Class {  // matrices of one shape

@@ -143,7 +143,6 @@ __global__ void __launch_bounds__(kEltThreads)
   double sum = 0;
   const bool mom = it.mom != nullptr;
   if (item_vec(it)) {
-    // four stretches at a time: their loads are under way together
     for (int64_t i0 = e0 + threadIdx.x * 8; i0 < e1; i0 += kEltThreads * 8 * kUnroll) {
       F8 g[kUnroll], m[kUnroll];
 #pragma unroll
@@ -216,7 +215,7 @@ __global__ void __launch_bounds__(kEltThreads)
     pow2 = ldexpf(1.f, max(-126, min(120, 13 - ilogb(norm))));
     unit = (float)(1.0 / ((norm + eps) * (double)pow2));
   }
-  if (chunk == 0 && threadIdx.x == 0) *it.scale = Scale{pow2, unit};
+  if (chunk == 0 && threadIdx.x == 0) *it.scale = Scale{unit};
   const int64_t e0 = chunk * it.chunk_elems, e1 = min(it.n, e0 + it.chunk_elems);
   const bool mom = it.mom != nullptr;
   // element i's place in the scaled matrix, whose lines are padded to ld

@@ -2,14 +2,15 @@
 // read once.
 //
 // A tile of the product engine has 256 rows; with one token its matrix instructions would work
-// on zeros, and its copies, one stage at a time and CTA pair, reach some 3 TB/s (36 to 39 us
-// at 4096 > 14336, bf16, for 1 to 8 tokens). Here every lane has several 16-byte loads of B under
-// way, which is what HBM asks for: 21.5 us for one token (5.5 TB/s), 23 us for two, 36 us for
-// four, where a lane's arithmetic takes over (4096 > 4096: 8.6, 9.5 and 12.4 us, the tiles 24);
+// on zeros, and its copies, one stage at a time and CTA pair, reach some 3.4 TB/s (35 us
+// at 4096 > 14336, bf16, for 8 tokens). Here every lane has several 16-byte loads of B under
+// way, which is what HBM asks for: 20.5 us for one token (5.7 TB/s), 22 us for two, 35.5 us for
+// four, where a lane's arithmetic takes over (4096 > 4096: 8.4, 9.4 and 12.3 us, the tiles 23);
 // beyond, the tiles are faster. Two forms, by which dimension of B is contiguous:
 //   k_few_rows: the sum's (an output by input weight): a warp takes four rows of B;
 //   k_few_cols: the result's: a lane takes eight columns, the sum is split over the warps of a
-//               block and over blocks, and k_few_finish adds the blocks' parts in order.
+//               block and over blocks, and k_few_finish adds the blocks' parts in order (4096 >
+//               14336: 25 us for one token, 26.5 for two, 43.5 for four).
 #pragma once
 
 #include "ta_mx_elementwise.cuh"

@@ -55,7 +55,6 @@ constexpr size_t kProductSmem = 1024 + kOperandSpace + kEpiWarps * kBlockBytes +
 // Per-matrix scale of a Newton-Schulz list: the stored fp16 input times `unit` is the
 // normalised matrix (unit is NaN where the input holds a NaN or an infinity).
 struct Scale {
-  float pow2;  // stored = input * pow2
   float unit;
 };
 
@@ -150,7 +149,7 @@ __device__ __forceinline__ Unit locate(const View& v, int u, int p_hint) {
   return w;
 }
 
-// K blocks [*k0, *k1) of a split. (At most 32 splits of at most 2^25 blocks: 32 bits suffice.)
+// K blocks [*k0, *k1) of a split. (At most 16 splits of at most 2^26 blocks: 32 bits suffice.)
 __device__ __forceinline__ void split_range(const Problem& P, int parts, int split, int* k0,
                                             int* k1) {
   const uint32_t total = (uint32_t)(P.kblocks * parts);
@@ -168,11 +167,12 @@ enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4
 // y = act(z), d = act'(z). A NaN z gives NaN for both.
 //
 // An epilogue has two warps a scheduler, so a call with branches inside (erfcf, the full forms of
-// expf and of the division) leaves its latency bare: with these 8192 x 512 > 4096 takes 54, 58 and
-// 62 us for SiLU, tanh-GELU and GELU, with those it took 104, 186 and 96 (34 without activation).
-// The forms here have no branch, use the hardware's exponential and reciprocal (__expf, __fdividef:
-// a few 1e-7 of a sigmoid or of Phi, under 1/500 of an fp16's rounding), and saturate by
-// themselves: exp(-z) = inf gives a sigmoid of 0.
+// expf and of the division) leaves its latency bare: with these 8192 x 512 > 4096 takes 51, 55 and
+// 61 us for SiLU, tanh-GELU and GELU, with those it took 104, 186 and 96 (32 without activation).
+// The forms here have no branch, use the hardware's exponential and reciprocal (__expf,
+// __fdividef), and saturate by themselves: exp(-z) = inf gives a sigmoid of 0. Relative to a sigmoid
+// or a Phi they are off by a few 1e-7 where it is not small; the exponential's error grows with its
+// argument, to some 1e-5 of a Phi of 1e-19 at z = -9, still 1/40 of an fp16's rounding.
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 // exp(u^2 / 2) Phi(-u) for u >= 0, Hastings' form: a polynomial in t = 1 / (1 + p u) without a
 // constant term. Its coefficients are a least-maximum fit of the relative error: 4e-7 up to u = 9
@@ -223,8 +223,10 @@ __device__ __forceinline__ void activate(int act, float z, float* y, float* d) {
 // by at most 2^-15, and relative to itself by at most 2^-9 for bf16 (down to 2^-93; beyond, by
 // 2^-102) and 2^-12 for fp16 (down to 2^-13; beyond, by 2^-25, half a step of fp16's own smallest
 // numbers): half of what rounding dz to the type costs next, in the activations' far negative tails
-// too. (Steps of 2^-14 throughout left SiLU' 10 % off at -12 and zero from -13 on, in the same time:
-// 75 us for 8192 x 512 > 4096 with SiLU.)
+// too. (Steps of 2^-14 throughout left SiLU' 10 % off at -12 and zero from -13 on. They took as
+// long in the forward pass, 75 us for 8192 x 512 > 4096 with SiLU, and 1 to 2 us less in a backward
+// pass: both together 73 us against 74.5 for 9714 x 1920 > 256, 32.2 against 33.6 for 777 x 1001 >
+// 1003.)
 // Codes: [0, kDerivCodes) the floating ones in order, then the steps; kDerivNeg is added for a
 // negative number, and what a NaN leaves in the low bits (0xffff of the one NaN that arithmetic
 // gives) stands for NaN.

@@ -53,6 +53,13 @@ class Muon(Optimizer):
     "original" (default) sqrt(max(1, rows / cols)), "match_rms_adamw"
     0.2 sqrt(max(rows, cols)).
 
+    The arguments are those of ``torch.optim.Muon``; the arithmetic differs in that
+    u is divided by |u|_F + eps (there max(|u|_F, eps)) and that the products
+    take fp16 operands (there bf16). Parameters of more than two dimensions are
+    stacks of matrices here: give a convolution's weight as a
+    [out, in * height * width] view. ``ns_coefficients`` are limited as
+    :func:`turboadam_b200.orthogonalize` says.
+
     Parameters: float32, bfloat16 or float16, at least two dimensions; the
     last two are the matrix. The momentum is kept in ``momentum_dtype``
     (float32 by default; bfloat16 halves it). u is rounded once to fp16
